@@ -879,6 +879,194 @@ m3_status m3_cuda_abs_max_static(int device, void *stream, m3_dtype dtype,
                                  size_t tensor_count, float *maxima,
                                  m3_error *error);
 
+/* ------------------------------------------------------------------------
+ * Serving operators: one step of a language model around its products
+ * ------------------------------------------------------------------------
+ * No counterpart in the reference.  A graph's shapes are fixed when its
+ * session is created; the rows, sequences and drafts of a serving step change
+ * with every step.  These calls therefore take device addresses and sizes,
+ * like m3_cuda_abs_max_static, and are stream-ordered: they check their
+ * arguments on the host, enqueue on `stream` (a cudaStream_t of the device;
+ * NULL is the legacy default stream) and return without waiting.  They
+ * allocate nothing and may be captured into a CUDA graph.  The calling
+ * thread's current device is restored before return.  Memory that they name
+ * must stay valid until the stream has passed the call; work on other streams
+ * is ordered by the caller's events.  A refused call enqueues nothing and
+ * writes nothing.
+ *
+ * 8-bit values are E4M3 (one sign, four exponent and three significand bits,
+ * largest value 448, no infinity), quantised in groups that share one F32
+ * scale:
+ *   a = max |v_i|,   scale = max(a / 448, 2^-126),   code_i = E4M3(v_i / scale)
+ * in F32, the quotient rounded to F32 and then to the nearest E4M3 value (ties
+ * to even).  The value that a code stands for is code * scale.  A group that
+ * holds a NaN or an infinity has a NaN scale and NaN codes (0x7f), so it reads
+ * back as NaN; a group of zeros has the scale 2^-126. */
+
+/* RMS norm into E4M3, with the residual's addition:
+ *   h = input, or input + residual rounded to `dtype`,
+ *   y = h * scale / sqrt(mean(h^2) + epsilon)     (F32; the mean over the row)
+ * and each `group` consecutive elements of a row of y quantised together.
+ * The row sums run in F32 in a fixed order of their own (not the reference's
+ * left-to-right order of M3_OP_RMS_NORM), so results repeat bit for bit.
+ * `sum` (may be NULL) receives h.  It may be the very tensor `input` or
+ * `residual` (same address and row stride); no other output may overlap an
+ * input or another output (M3_STATUS_INVALID_ARGUMENT; the byte spans are
+ * compared).  Rows of zero `width` are refused; zero `rows` do nothing. */
+typedef struct {
+    const void *input;           /* [rows, width] of dtype */
+    const void *residual;        /* [rows, width] of dtype, or NULL */
+    void *sum;                   /* [rows, width] of dtype, or NULL; needs a
+                                    residual */
+    m3_dtype dtype;              /* F32, F16 or BF16 */
+    uint64_t input_stride;       /* elements from row to row (0: width) */
+    uint64_t residual_stride;
+    uint64_t sum_stride;
+    const void *scale;           /* [width] of scale_dtype: the norm's weight */
+    m3_dtype scale_dtype;        /* F32, F16 or BF16 */
+    uint64_t rows;
+    uint64_t width;
+    uint64_t group;              /* elements per code scale, a divisor of
+                                    width (0: width, one scale per row) */
+    float epsilon;               /* finite and positive */
+    void *codes;                 /* [rows, width] E4M3, dense */
+    float *code_scales;          /* [rows, width / group], dense */
+} m3_cuda_rms_norm_e4m3_args;
+
+void m3_cuda_rms_norm_e4m3_args_init(m3_cuda_rms_norm_e4m3_args *args);
+m3_status m3_cuda_rms_norm_e4m3(int device, void *stream,
+                                const m3_cuda_rms_norm_e4m3_args *args,
+                                m3_error *error);
+
+/* A paged key/value cache in E4M3.  A page holds page_tokens slots, a slot one
+ * token's keys and values: for each of `heads` heads a vector of head_dim
+ * codes and one scale.  The cache owns its device memory, zero when created:
+ *   codes  [pages, page_tokens, heads, head_dim] E4M3   (keys, then values)
+ *   scales [pages, page_tokens, heads] F32              (keys, then values)
+ * Which pages belong to which sequence is the caller's page table. */
+typedef struct m3_cuda_cache m3_cuda_cache;
+
+typedef struct {
+    int device;                  /* CUDA ordinal, or M3_CUDA_DEVICE_CURRENT */
+    uint64_t pages;
+    uint32_t page_tokens;
+    uint32_t heads;
+    uint32_t head_dim;
+} m3_cuda_cache_options;
+
+m3_status m3_cuda_cache_create(m3_cuda_cache **cache,
+                               const m3_cuda_cache_options *options,
+                               m3_error *error);
+/* Waits for the device's work before it frees the memory. */
+void m3_cuda_cache_free(m3_cuda_cache *cache);
+
+/* A batch of sequences, their tokens packed one sequence after another: row t
+ * belongs to the sequence s with offsets[s] <= t < offsets[s + 1] and is its
+ * token number p = starts[s] + t - offsets[s], which lies in slot
+ * p % page_tokens of page page_table[s * page_table_stride + p / page_tokens].
+ * All arrays are device memory, read when the stream reaches the call.
+ * Sequences may be empty; rows before offsets[0], at or behind
+ * offsets[sequences], or at or behind `rows` are not touched, nor is what
+ * they would name.
+ *
+ * A row whose position is negative or behind the page table's row, or whose
+ * page is outside the cache, is skipped; the cache remembers the first such
+ * row, and m3_cuda_cache_synchronize reports it. */
+typedef struct {
+    const int32_t *page_table;   /* [sequences, page_table_stride] */
+    uint64_t page_table_stride;  /* pages listed for each sequence */
+    const int32_t *offsets;      /* [sequences + 1], not decreasing */
+    const int32_t *starts;       /* [sequences], or NULL: all 0 */
+    uint64_t sequences;
+    uint64_t rows;               /* rows that the key and value tensors have,
+                                    at most INT32_MAX */
+} m3_cuda_cache_batch;
+
+/* The keys or the values of a batch: [rows, heads, head_dim], the vectors'
+ * elements contiguous, so that a fused projection's columns can be named
+ * where they lie. */
+typedef struct {
+    void *data;
+    m3_dtype dtype;              /* F32, F16 or BF16 */
+    uint64_t token_stride;       /* elements (0: heads * head_dim) */
+    uint64_t head_stride;        /* elements (0: head_dim) */
+} m3_cuda_cache_rows;
+
+/* Quantise the rows' keys and values into their slots; each vector of head_dim
+ * elements is one group.  No two rows of a call may name one slot, nor may
+ * calls that overlap in time name a slot that one of them writes: its vectors
+ * are then unspecified (all other slots hold what they should). */
+m3_status m3_cuda_cache_write(m3_cuda_cache *cache, void *stream,
+                              const m3_cuda_cache_batch *batch,
+                              const m3_cuda_cache_rows *keys,
+                              const m3_cuda_cache_rows *values,
+                              m3_error *error);
+/* Read the rows' slots back: code * scale, in F32, rounded to the rows' dtype.
+ * Several rows may name one slot (a shared prefix).  The vectors of `keys` and
+ * `values` must not overlap each other (they may interleave). */
+m3_status m3_cuda_cache_read(m3_cuda_cache *cache, void *stream,
+                             const m3_cuda_cache_batch *batch,
+                             const m3_cuda_cache_rows *keys,
+                             const m3_cuda_cache_rows *values,
+                             m3_error *error);
+
+/* Wait for `stream`, then report (and forget) the first skipped row since the
+ * last report: M3_STATUS_OUT_OF_RANGE, with the row and the reason in the
+ * message. */
+m3_status m3_cuda_cache_synchronize(m3_cuda_cache *cache, void *stream,
+                                    m3_error *error);
+
+/* The cache's arrays (see above), e.g. for an attention kernel that reads the
+ * codes, or to copy pages.  Any output may be NULL. */
+m3_status m3_cuda_cache_device_pointers(const m3_cuda_cache *cache,
+                                        void **key_codes, float **key_scales,
+                                        void **value_codes,
+                                        float **value_scales, m3_error *error);
+
+/* Verification of drafted tokens.  For each sequence, drafts i = 0, 1, ... are
+ * accepted while
+ *   uniforms[i] * draft_i(token_i) < target_i(token_i)
+ * (the product exact), up to the sequence's length.  One more token is drawn
+ * behind the m accepted ones with uniforms[drafts]: from max(target_m -
+ * draft_m, 0) after a rejection (from target_m where that is zero for every
+ * token), from target_m where all drafts were accepted.  The drawn token is
+ * the first whose running sum of weights exceeds uniform * total, the sums in
+ * 64 bits.  So the tokens are distributed as the target's own.  Without
+ * `draft` the drafts were not drawn but given: draft_i is 1 at token_i and 0
+ * elsewhere.
+ *
+ * Row strides let a padded vocabulary be named as it lies; all other arrays
+ * are dense.  Only what the rule needs is read: the drafts up to the first
+ * rejection, then one row of each model.
+ *
+ * One bad sequence does not fail its batch: a sequence whose length is outside
+ * [0, drafts] (e.g. -1 for a padded place), or that needs a token outside the
+ * vocabulary, a uniform outside [0, 1), a probability that is negative, NaN or
+ * infinite, or a row without a positive one, gets accepted = -1 and the token
+ * -1 everywhere.  No output may overlap an input or the other output. */
+typedef struct {
+    const void *target;          /* [batch, drafts + 1, vocabulary] of dtype */
+    const void *draft;           /* [batch, drafts, vocabulary] of dtype, or
+                                    NULL */
+    m3_dtype dtype;              /* F32, F16 or BF16 */
+    uint64_t target_stride;      /* elements from row to row (0: vocabulary) */
+    uint64_t draft_stride;
+    const int32_t *draft_tokens; /* [batch, drafts] */
+    const int32_t *lengths;      /* [batch] drafts in use, or NULL: all */
+    const float *uniforms;       /* [batch, drafts + 1], in [0, 1) */
+    uint64_t batch;
+    uint64_t drafts;             /* may be 0: one token is drawn */
+    uint64_t vocabulary;         /* 1 to INT32_MAX */
+    int32_t *tokens;             /* [batch, drafts + 1]: the accepted drafts,
+                                    the drawn token, then -1 */
+    int32_t *accepted;           /* [batch]: drafts accepted, or -1 */
+} m3_cuda_verify_draft_args;
+
+void m3_cuda_verify_draft_args_init(m3_cuda_verify_draft_args *args);
+m3_status m3_cuda_verify_draft(int device, void *stream,
+                               const m3_cuda_verify_draft_args *args,
+                               m3_error *error);
+
 #ifdef __cplusplus
 }
 #endif

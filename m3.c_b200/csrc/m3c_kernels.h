@@ -216,6 +216,81 @@ typedef struct {
 
 int m3c_launch_categorical(const m3c_categorical_params *params, void *stream);
 
+/* RMS norm into E4M3 codes (m3_cuda_rms_norm_e4m3). */
+typedef struct {
+    const void *x;
+    const void *resid_b;        /* NULL: none */
+    void *sum_out;              /* NULL: none */
+    uint64_t x_stride;          /* elements from row to row */
+    uint64_t resid_stride;
+    uint64_t sum_stride;
+    const void *scale;          /* [width] */
+    void *codes;                /* dense [rows, width] E4M3 */
+    float *code_scales;         /* dense [rows, width / group] */
+    uint64_t rows;
+    uint64_t width;
+    uint64_t group;
+    int32_t dtype;              /* x, resid_b, sum_out */
+    int32_t scale_dtype;
+    float epsilon;
+    uint32_t skip_before;       /* session launches: as in m3c_norm_params */
+    m3c_status *status;         /* NULL: a direct call */
+    int32_t first_of_run;
+    int32_t reserved;
+} m3c_norm_e4m3_params;
+
+int m3c_launch_norm_e4m3(const m3c_norm_e4m3_params *params, void *stream);
+
+/* Rows of a paged E4M3 cache, written (quantised) or read back. */
+typedef struct {
+    uint8_t *codes[2];          /* keys, values */
+    float *scales[2];
+    void *rows[2];
+    uint64_t token_stride[2];   /* elements */
+    uint64_t head_stride[2];
+    int32_t dtype[2];
+    const int32_t *page_table;
+    const int32_t *offsets;
+    const int32_t *starts;      /* NULL: 0 */
+    uint64_t page_table_stride;
+    uint64_t pages;
+    uint32_t sequences;
+    uint32_t row_count;
+    uint32_t page_tokens;
+    uint32_t heads;
+    uint32_t head_dim;
+    uint32_t reserved;
+    unsigned long long *first_skipped;  /* row * 4 + reason, or all ones */
+} m3c_cache_params;
+
+#define M3C_CACHE_BAD_POSITION 1U
+#define M3C_CACHE_BAD_PAGE 2U
+
+int m3c_launch_cache_write(const m3c_cache_params *params, void *stream);
+int m3c_launch_cache_read(const m3c_cache_params *params, void *stream);
+
+/* Verification of drafted tokens (m3_cuda_verify_draft). */
+typedef struct {
+    const void *target;
+    const void *draft;          /* NULL: each draft had probability one */
+    uint64_t target_stride;     /* elements from row to row */
+    uint64_t draft_stride;
+    const int32_t *draft_tokens;
+    const int32_t *lengths;     /* NULL: `drafts` each */
+    const float *uniforms;
+    int32_t *tokens;
+    int32_t *accepted;
+    uint64_t batch;
+    uint64_t drafts;
+    uint32_t vocabulary;
+    int32_t dtype;
+    m3c_status *status;         /* NULL: a direct call */
+    uint32_t skip_before;
+    int32_t first_of_run;
+} m3c_verify_params;
+
+int m3c_launch_verify(const m3c_verify_params *params, void *stream);
+
 /* The warp-specialised SOFTMAX/TOP_K(k <= 1)/ROW_SUM pipeline for F32 rows of
  * 512 or 1024 elements (m3c_ring.cu); -1 when it does not apply. */
 int m3c_launch_softmax_ring(const m3c_softmax_params *params, void *stream);

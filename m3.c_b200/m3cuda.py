@@ -219,6 +219,61 @@ class Command(ctypes.Structure):
     _fields_ = [("kind", ctypes.c_int), ("descriptor", _Descriptor)]
 
 
+# serving operators
+class RmsNormE4m3Args(ctypes.Structure):
+    """m3_cuda_rms_norm_e4m3_args; pointers are device addresses."""
+
+    _fields_ = [("input", ctypes.c_void_p), ("residual", ctypes.c_void_p),
+                ("sum", ctypes.c_void_p), ("dtype", ctypes.c_int),
+                ("input_stride", ctypes.c_uint64),
+                ("residual_stride", ctypes.c_uint64),
+                ("sum_stride", ctypes.c_uint64), ("scale", ctypes.c_void_p),
+                ("scale_dtype", ctypes.c_int), ("rows", ctypes.c_uint64),
+                ("width", ctypes.c_uint64), ("group", ctypes.c_uint64),
+                ("epsilon", ctypes.c_float), ("codes", ctypes.c_void_p),
+                ("code_scales", ctypes.c_void_p)]
+
+    def __init__(self, **fields):
+        super().__init__(**{"epsilon": 1e-6, **fields})
+
+
+class VerifyDraftArgs(ctypes.Structure):
+    """m3_cuda_verify_draft_args; pointers are device addresses."""
+
+    _fields_ = [("target", ctypes.c_void_p), ("draft", ctypes.c_void_p),
+                ("dtype", ctypes.c_int), ("target_stride", ctypes.c_uint64),
+                ("draft_stride", ctypes.c_uint64),
+                ("draft_tokens", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
+                ("uniforms", ctypes.c_void_p), ("batch", ctypes.c_uint64),
+                ("drafts", ctypes.c_uint64), ("vocabulary", ctypes.c_uint64),
+                ("tokens", ctypes.c_void_p), ("accepted", ctypes.c_void_p)]
+
+
+class CacheOptions(ctypes.Structure):
+    _fields_ = [("device", ctypes.c_int), ("pages", ctypes.c_uint64),
+                ("page_tokens", ctypes.c_uint32), ("heads", ctypes.c_uint32),
+                ("head_dim", ctypes.c_uint32)]
+
+
+class CacheBatch(ctypes.Structure):
+    """m3_cuda_cache_batch: the sequences of a cache write or read, as device
+    int32 arrays (page_table, offsets, starts or None)."""
+
+    _fields_ = [("page_table", ctypes.c_void_p),
+                ("page_table_stride", ctypes.c_uint64),
+                ("offsets", ctypes.c_void_p), ("starts", ctypes.c_void_p),
+                ("sequences", ctypes.c_uint64), ("rows", ctypes.c_uint64)]
+
+
+class CacheRows(ctypes.Structure):
+    """m3_cuda_cache_rows: the keys or values of a batch (device address,
+    dtype, strides in elements; 0: dense)."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("dtype", ctypes.c_int),
+                ("token_stride", ctypes.c_uint64),
+                ("head_stride", ctypes.c_uint64)]
+
+
 STORAGE_DATA = ctypes.CFUNCTYPE(ctypes.c_void_p, ctypes.c_void_p)
 
 
@@ -401,6 +456,32 @@ _CUDA_SIGNATURES = {
         ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
         ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(ctypes.c_uint64),
         ctypes.c_size_t, ctypes.c_void_p, ctypes.POINTER(M3Error)]),
+    "m3_cuda_rms_norm_e4m3_args_init": (None, [ctypes.POINTER(RmsNormE4m3Args)]),
+    "m3_cuda_rms_norm_e4m3": (ctypes.c_int, [
+        ctypes.c_int, ctypes.c_void_p, ctypes.POINTER(RmsNormE4m3Args),
+        ctypes.POINTER(M3Error)]),
+    "m3_cuda_verify_draft_args_init": (None, [ctypes.POINTER(VerifyDraftArgs)]),
+    "m3_cuda_verify_draft": (ctypes.c_int, [
+        ctypes.c_int, ctypes.c_void_p, ctypes.POINTER(VerifyDraftArgs),
+        ctypes.POINTER(M3Error)]),
+    "m3_cuda_cache_create": (ctypes.c_int, [
+        ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(CacheOptions),
+        ctypes.POINTER(M3Error)]),
+    "m3_cuda_cache_free": (None, [ctypes.c_void_p]),
+    "m3_cuda_cache_write": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.POINTER(CacheBatch),
+        ctypes.POINTER(CacheRows), ctypes.POINTER(CacheRows),
+        ctypes.POINTER(M3Error)]),
+    "m3_cuda_cache_read": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.POINTER(CacheBatch),
+        ctypes.POINTER(CacheRows), ctypes.POINTER(CacheRows),
+        ctypes.POINTER(M3Error)]),
+    "m3_cuda_cache_synchronize": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.POINTER(M3Error)]),
+    "m3_cuda_cache_device_pointers": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p),
+        ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(ctypes.c_void_p),
+        ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(M3Error)]),
 }
 
 
@@ -831,3 +912,69 @@ def abs_max_static(dtype: int, pointers, counts, maxima: int, device: int = 0,
     err = M3Error()
     check(load().m3_cuda_abs_max_static(device, stream, dtype, inputs, sizes,
                                         n, maxima, ctypes.byref(err)), err)
+
+
+def rms_norm_e4m3(args: RmsNormE4m3Args, device: int = 0, stream: int = 0) -> None:
+    """m3_cuda_rms_norm_e4m3: enqueue the RMS norm (with its residual's
+    addition) into E4M3 codes and scales on `stream`; see include/m3_cuda.h."""
+    err = M3Error()
+    check(load().m3_cuda_rms_norm_e4m3(device, stream, args, err), err)
+
+
+def verify_draft(args: VerifyDraftArgs, device: int = 0, stream: int = 0) -> None:
+    """m3_cuda_verify_draft: enqueue the verification of drafted tokens on
+    `stream`; see include/m3_cuda.h."""
+    err = M3Error()
+    check(load().m3_cuda_verify_draft(device, stream, args, err), err)
+
+
+class Cache:
+    """m3_cuda_cache: a paged key/value cache in E4M3 (include/m3_cuda.h)."""
+
+    def __init__(self, pages: int, page_tokens: int, heads: int, head_dim: int,
+                 device: int = -1):
+        self.lib = load()
+        self.handle = ctypes.c_void_p()
+        self.shape = (pages, page_tokens, heads, head_dim)
+        options = CacheOptions(device, pages, page_tokens, heads, head_dim)
+        err = M3Error()
+        check(self.lib.m3_cuda_cache_create(ctypes.byref(self.handle), options,
+                                            err), err)
+
+    def close(self) -> None:
+        if self.handle:
+            self.lib.m3_cuda_cache_free(self.handle)
+            self.handle = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def write(self, batch: CacheBatch, keys: CacheRows, values: CacheRows,
+              stream: int = 0) -> None:
+        """Enqueue the quantisation of the batch's rows into their slots."""
+        err = M3Error()
+        check(self.lib.m3_cuda_cache_write(self.handle, stream, batch, keys,
+                                           values, err), err)
+
+    def read(self, batch: CacheBatch, keys: CacheRows, values: CacheRows,
+             stream: int = 0) -> None:
+        """Enqueue the read of the batch's slots into dense rows."""
+        err = M3Error()
+        check(self.lib.m3_cuda_cache_read(self.handle, stream, batch, keys,
+                                          values, err), err)
+
+    def synchronize(self, stream: int = 0) -> None:
+        """Wait for `stream`; raises M3Failure for the first skipped row."""
+        err = M3Error()
+        check(self.lib.m3_cuda_cache_synchronize(self.handle, stream, err), err)
+
+    def pointers(self) -> tuple[int, int, int, int]:
+        """Device addresses: key codes, key scales, value codes, value scales."""
+        out = [ctypes.c_void_p() for _ in range(4)]
+        err = M3Error()
+        check(self.lib.m3_cuda_cache_device_pointers(
+            self.handle, *(ctypes.byref(p) for p in out), err), err)
+        return tuple(p.value or 0 for p in out)
