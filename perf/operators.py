@@ -297,9 +297,10 @@ def _package():
 
 
 class _Device:
-    """Device memory at `pointer` as torch sees other libraries' arrays."""
+    """Device memory at `pointer` as torch sees other libraries' arrays; its owner lives as long as a tensor over it."""
 
-    def __init__(self, pointer, shape, kind):
+    def __init__(self, owner, pointer, shape, kind):
+        self.owner = owner
         self.__cuda_array_interface__ = {"data": (pointer, False), "shape": tuple(shape), "typestr": kind,
                                          "version": 2}
 
@@ -336,9 +337,9 @@ def _own_prepare(s):
         shape = (s["pages"], case["page"], heads)
         views = {}
         for name, pointers in zip(("key", "value"), (cache.pointers()[:2], cache.pointers()[2:])):
-            codes = torch.as_tensor(_Device(pointers[0], shape + (dim,), "|u1"), device="cuda")
+            codes = torch.as_tensor(_Device(cache, pointers[0], shape + (dim,), "|u1"), device="cuda")
             views[name + "_codes"] = codes.view(torch.float8_e4m3fn)
-            views[name + "_scales"] = torch.as_tensor(_Device(pointers[1], shape, "<f4"), device="cuda")
+            views[name + "_scales"] = torch.as_tensor(_Device(cache, pointers[1], shape, "<f4"), device="cuda")
         for name, view in views.items():
             view.copy_(s.pop(name))
         s["cache"] = cache
