@@ -19,6 +19,7 @@
 namespace m3c {
 
 constexpr float E4M3_LARGEST = 448.0f;
+constexpr float E4M3_LARGEST_RECIPROCAL = 1.0f / 448.0f;
 constexpr float E4M3_SMALLEST_SCALE = 0x1p-126f;
 // div_markstein's remainder v - q s is a multiple of ulp(q) ulp(s).  Quotients
 // below 2^-10 have the code 0 however they round, and for the others the
@@ -35,7 +36,10 @@ __device__ __forceinline__ uint32_t magnitude_bits(float v)
 __device__ __forceinline__ float e4m3_scale(uint32_t largest_bits)
 {
     if (largest_bits >= 0x7f800000u) return as_float(0x7fc00000u);
-    return fmaxf(__fdiv_rn(as_float(largest_bits), E4M3_LARGEST), E4M3_SMALLEST_SCALE);
+    const float a = as_float(largest_bits);
+    const float s = a < E4M3_MARKSTEIN_SCALE ? __fdiv_rn(a, E4M3_LARGEST)
+                                             : div_markstein(a, E4M3_LARGEST, E4M3_LARGEST_RECIPROCAL);
+    return fmaxf(s, E4M3_SMALLEST_SCALE);
 }
 
 // The divisor of one group: its scale and the scale's rounded reciprocal, or a
@@ -60,9 +64,74 @@ __device__ __forceinline__ uint8_t e4m3_code(float v, const e4m3_divisor &d)
     return __nv_cvt_float_to_fp8(e4m3_quotient(v, d), __NV_SATFINITE, __NV_E4M3);
 }
 
+// The largest magnitude of N values, a NaN if one of them is a NaN.
+template <int N>
+__device__ __forceinline__ float largest_of(const float (&v)[N])
+{
+    static_assert(N % 2 == 0 || N == 1, "pairs");
+    if constexpr (N == 1) {
+        return fabsf(v[0]);
+    } else {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; i += 2) asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(m), "f"(v[i]), "f"(v[i + 1]));
+        return m;
+    }
+}
+
+// Store the codes of eight values (to an 8-byte boundary) or of one.
+template <int N>
+__device__ __forceinline__ void e4m3_store(uint8_t *to, const float (&v)[N], const e4m3_divisor &d)
+{
+    static_assert(N == 1 || N == 8, "one code or eight");
+    float q[N];
+    if (d.reciprocal == 0.0f) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) q[i] = __fdiv_rn(v[i], d.scale);
+    } else {
+        // div_markstein, two quotients a packed instruction
+        if constexpr (N == 1) {
+            q[0] = div_markstein(v[0], d.scale, d.reciprocal);
+        } else {
+            const uint64_t y = f2_splat(d.reciprocal);
+            const uint64_t s = f2_splat(-d.scale);
+#pragma unroll
+            for (int i = 0; i < N; i += 2) {
+                const uint64_t a = f2_pack(v[i], v[i + 1]);
+                const uint64_t q0 = f2_mul(a, y);
+                f2_unpack(f2_fma(f2_fma(q0, s, a), y, q0), q[i], q[i + 1]);
+            }
+        }
+    }
+    if constexpr (N == 1) {
+        *to = __nv_cvt_float_to_fp8(q[0], __NV_SATFINITE, __NV_E4M3);
+    } else {
+        uint32_t pair[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            pair[i] = __nv_cvt_float2_to_fp8x2(make_float2(q[2 * i], q[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+        }
+        *reinterpret_cast<uint2 *>(to) = make_uint2(pair[0] | (pair[1] << 16), pair[2] | (pair[3] << 16));
+    }
+}
+
 __device__ __forceinline__ float e4m3_value(uint8_t code)
 {
     return __half2float(__half(__nv_cvt_fp8_to_halfraw(code, __NV_E4M3)));
+}
+
+// The values of eight codes, exact.
+__device__ __forceinline__ void e4m3_values(const uint2 &codes, float (&x)[8])
+{
+    const uint32_t w[2] = {codes.x, codes.y};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2_raw two = __nv_cvt_fp8x2_to_halfraw2(
+            static_cast<__nv_fp8x2_storage_t>(w[i / 2] >> (i % 2 * 16)), __NV_E4M3);
+        const float2 f = __half22float2(__half2(two));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+    }
 }
 
 // Element i of a float tensor, and its store.
