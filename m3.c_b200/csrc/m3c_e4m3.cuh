@@ -79,6 +79,20 @@ __device__ __forceinline__ float largest_of(const float (&v)[N])
     }
 }
 
+// The codes of four quotients, the first in the lowest byte; NaN becomes 0x7f,
+// magnitudes above 448 (a rounding step at most) become 448.
+__device__ __forceinline__ uint32_t e4m3_four(const float *q)
+{
+    uint32_t codes;
+    asm("{\n\t.reg .b16 low, high;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 low, %2, %1;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 high, %4, %3;\n\t"
+        "mov.b32 %0, {low, high};\n\t}"
+        : "=r"(codes)
+        : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]));
+    return codes;
+}
+
 // Store the codes of eight values (to an 8-byte boundary) or of one.
 template <int N>
 __device__ __forceinline__ void e4m3_store(uint8_t *to, const float (&v)[N], const e4m3_divisor &d)
@@ -106,12 +120,7 @@ __device__ __forceinline__ void e4m3_store(uint8_t *to, const float (&v)[N], con
     if constexpr (N == 1) {
         *to = __nv_cvt_float_to_fp8(q[0], __NV_SATFINITE, __NV_E4M3);
     } else {
-        uint32_t pair[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            pair[i] = __nv_cvt_float2_to_fp8x2(make_float2(q[2 * i], q[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
-        }
-        *reinterpret_cast<uint2 *>(to) = make_uint2(pair[0] | (pair[1] << 16), pair[2] | (pair[3] << 16));
+        *reinterpret_cast<uint2 *>(to) = make_uint2(e4m3_four(q), e4m3_four(q + 4));
     }
 }
 

@@ -10,8 +10,6 @@
 #include "m3c_e4m3.cuh"
 #include "m3c_kernels.h"
 
-extern "C" void m3c_fastdiv_init(m3c_fastdiv *fd, uint32_t divisor);
-
 namespace m3c {
 namespace {
 
@@ -35,14 +33,20 @@ __device__ __forceinline__ uint32_t warp_max(uint32_t v)
     return __reduce_max_sync(0xffffffffu, v);
 }
 
-unsigned capped_grid(uint64_t wanted, unsigned per_sm)
+// SMs of the current device.
+int sm_count()
 {
     int device = 0;
     int sms = 148;
     if (cudaGetDevice(&device) == cudaSuccess) {
         cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
     }
-    const uint64_t cap = static_cast<uint64_t>(sms) * per_sm;
+    return sms;
+}
+
+unsigned capped_grid(uint64_t wanted, unsigned per_sm)
+{
+    const uint64_t cap = static_cast<uint64_t>(sm_count()) * per_sm;
     // at least one CTA: an empty launch still records the start of the run
     return static_cast<unsigned>(wanted == 0 ? 1 : (wanted < cap ? wanted : cap));
 }
@@ -101,7 +105,9 @@ __device__ __forceinline__ Piece<DT, VEC> load_piece(const void *base, uint64_t 
     return v;
 }
 
-template <int DT, int VEC>
+// WIDE: a 32-byte piece (to a 32-byte boundary) in one store, which fills its
+// sector at once.
+template <int DT, int VEC, bool WIDE = false>
 __device__ __forceinline__ void store_piece(void *base, uint64_t element, const Piece<DT, VEC> &v)
 {
     char *to = static_cast<char *>(base) + element * (DT == M3C_F32 ? 4u : 2u);
@@ -109,6 +115,10 @@ __device__ __forceinline__ void store_piece(void *base, uint64_t element, const 
         *reinterpret_cast<uint16_t *>(to) = static_cast<uint16_t>(v.w[0]);
     } else if constexpr (Piece<DT, VEC>::BYTES == 4) {
         *reinterpret_cast<uint32_t *>(to) = v.w[0];
+    } else if constexpr (Piece<DT, VEC>::BYTES == 32 && WIDE) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v.w[0]), "r"(v.w[1]),
+                     "r"(v.w[2]), "r"(v.w[3]), "r"(v.w[4]), "r"(v.w[5]), "r"(v.w[6]), "r"(v.w[7])
+                     : "memory");
     } else {
 #pragma unroll
         for (int i = 0; i < Piece<DT, VEC>::WORDS / 4; ++i) {
@@ -254,8 +264,15 @@ __device__ __forceinline__ void multiply(float (&a)[N], float b)
     multiply(a, all);
 }
 
+// The most threads of a row: the register kernel's widest rows are VEC * K times
+// as many elements.
+constexpr int norm_block(int vec, int k)
+{
+    return vec == 1 ? 512 : k == 1 ? 1024 : k == 2 ? 512 : 256;
+}
+
 template <int DT, int MODE, int VEC, int K>
-__global__ void __launch_bounds__(K == 1 ? 1024 : 512, K == 4 && DT != M3C_F32 ? 2 : 1)
+__global__ void __launch_bounds__(norm_block(VEC, K))
     norm_e4m3_kernel(const __grid_constant__ m3c_norm_e4m3_params p)
 {
     extern __shared__ uint32_t words[];  // GROUP_WORDS: the groups' maxima of |z|, row by row
@@ -375,7 +392,7 @@ __global__ void __launch_bounds__(K == 1 ? 1024 : 512, K == 4 && DT != M3C_F32 ?
     }
     if (!live) return;
     const float inverse = __frsqrt_rn(__fadd_rn(__fdiv_rn(squares[0], static_cast<float>(width)), p.epsilon));
-    e4m3_divisor d;
+    e4m3_divisor d = {};
     if constexpr (MODE == GROUP_ROW) {
         d = e4m3_divide_by(e4m3_scale(magnitude_bits(__fmul_rn(as_float(largest), inverse))));
         if (tid == 0) p.code_scales[row] = d.scale;
@@ -386,9 +403,9 @@ __global__ void __launch_bounds__(K == 1 ? 1024 : 512, K == 4 && DT != M3C_F32 ?
         const uint32_t at = (k * threads + tid) * VEC;
         if (at >= width) continue;
         if constexpr (MODE != GROUP_ROW) {
-            if constexpr (MODE == GROUP_WORDS) most[k] = as_float(words[place + group_of(at)]);
-            d = e4m3_divide_by(e4m3_scale(magnitude_bits(__fmul_rn(most[k], inverse))));
             const uint32_t g = group_of(at);
+            if constexpr (MODE == GROUP_WORDS) most[k] = as_float(words[place + g]);
+            d = e4m3_divide_by(e4m3_scale(magnitude_bits(__fmul_rn(most[k], inverse))));
             if (at == g * group) p.code_scales[row * groups + g] = d.scale;
         }
         multiply(z[k], inverse);
@@ -493,13 +510,13 @@ int norm_depth(const m3c_norm_e4m3_params &p, bool vectors, cudaStream_t stream)
 {
     if (!vectors) return norm_launch<DT, MODE, 1, 16>(p, stream);
     // pieces per thread: two keep a row of 4096 elements in 256 threads; wider
-    // rows take four, unless there are too few rows to fill the SMs with
+    // rows take more, unless there are too few rows to fill the SMs with
     // their fewer threads
     const uint64_t pieces = p.width / 8u;
-    const int k = pieces <= 32u ? 1 : pieces <= 512u || (pieces <= 1024u && p.rows < 2048u) ? 2 : 4;
-    if (k == 1) return norm_launch<DT, MODE, 8, 1>(p, stream);
-    if (k == 2) return norm_launch<DT, MODE, 8, 2>(p, stream);
-    return norm_launch<DT, MODE, 8, 4>(p, stream);
+    if (pieces <= 32u) return norm_launch<DT, MODE, 8, 1>(p, stream);
+    if (pieces <= 512u || (pieces <= 1024u && p.rows < 2048u)) return norm_launch<DT, MODE, 8, 2>(p, stream);
+    if (pieces <= 1024u) return norm_launch<DT, MODE, 8, 4>(p, stream);
+    return norm_launch<DT, MODE, 8, 8>(p, stream);
 }
 
 template <int DT>
@@ -514,136 +531,199 @@ int norm_mode(const m3c_norm_e4m3_params &p, bool vectors, cudaStream_t stream)
 // ------------------------------------------------------------------ cache
 
 // Where packed row t lies in the cache: its slot, or -1 where it has none (not
-// in a sequence, or skipped and recorded).
-__device__ int64_t cache_slot(const m3c_cache_params &p, uint32_t t)
+// in a sequence, or skipped and recorded).  `s` is the last sequence that
+// begins at or before t, if any does.
+__device__ __forceinline__ int64_t slot_in_sequence(const m3c_cache_params &p, uint32_t t, uint32_t s)
 {
-    // the last sequence that begins at or before t
-    if (static_cast<int64_t>(t) < p.offsets[0]) return -1;
-    uint32_t low = 0;
-    uint32_t high = p.sequences;
-    while (high - low > 1) {
-        const uint32_t middle = low + (high - low) / 2;
-        if (p.offsets[middle] <= static_cast<int64_t>(t)) {
-            low = middle;
-        } else {
-            high = middle;
-        }
-    }
-    if (static_cast<int64_t>(t) >= p.offsets[low + 1]) return -1;
-    const int64_t position =
-        (p.starts != nullptr ? static_cast<int64_t>(p.starts[low]) : 0) + t - p.offsets[low];
-    uint32_t reason = 0u;
-    int64_t slot = -1;
-    if (position < 0 || static_cast<uint64_t>(position) / p.page_tokens >= p.page_table_stride) {
-        reason = M3C_CACHE_BAD_POSITION;
-    } else {
-        const uint64_t at = static_cast<uint64_t>(position) / p.page_tokens;
-        const int64_t page = p.page_table[low * p.page_table_stride + at];
-        if (page < 0 || static_cast<uint64_t>(page) >= p.pages) {
+    const int64_t row = t;
+    const int64_t begin = p.offsets[s];
+    if (row < begin || row >= p.offsets[s + 1]) return -1;
+    const int64_t position = (p.starts != nullptr ? static_cast<int64_t>(p.starts[s]) : 0) + row - begin;
+    uint32_t reason = M3C_CACHE_BAD_POSITION;
+    // positions below 2^32 fit the 32-bit division
+    if (position >= 0) {
+        const uint32_t at = static_cast<uint32_t>(position) / p.page_tokens;
+        if (at < p.page_table_stride) {
+            const int64_t page = p.page_table[s * p.page_table_stride + at];
+            if (page >= 0 && static_cast<uint64_t>(page) < p.pages) {
+                return page * p.page_tokens + static_cast<int64_t>(static_cast<uint32_t>(position) - at * p.page_tokens);
+            }
             reason = M3C_CACHE_BAD_PAGE;
-        } else {
-            slot = page * p.page_tokens + static_cast<int64_t>(static_cast<uint64_t>(position) % p.page_tokens);
         }
     }
-    if (reason != 0u) atomicMin(p.first_skipped, static_cast<unsigned long long>(t) * 4u + reason);
-    return slot;
+    atomicMin(p.first_skipped, static_cast<unsigned long long>(t) * 4u + reason);
+    return -1;
 }
 
-// The vector kernel: vectors of a multiple of eight elements up to 256, rows
-// aligned for 16-byte accesses.  A vector belongs to `lanes` lanes (a power of
-// two), eight elements each; a CTA takes DEPTH * 256 / lanes consecutive
-// vectors, those of a row (keys, then values, head by head) beside one
-// another, and finds the slots of their rows once, in shared memory.  Bytes
-// bound both directions: three per element of 16-bit rows.
-#ifndef DW
-#define DW 4
-#endif
-#ifndef DR
-#define DR 4
-#endif
-constexpr int CACHE_DEPTH_WRITE = DW;
-constexpr int CACHE_DEPTH_READ = DR;
-constexpr int CACHE_DEPTH = CACHE_DEPTH_READ > CACHE_DEPTH_WRITE ? CACHE_DEPTH_READ : CACHE_DEPTH_WRITE;
-constexpr uint32_t CACHE_MOST_ROWS = QUANT_THREADS * CACHE_DEPTH / 2 + 2;  // of a CTA: one head, eight elements
+// The slots of `count` consecutive rows, by one warp: the sequence of the first
+// by a 32-way search, the others' from there on (the sequences of a CTA's few
+// rows are the same or next to one another).
+__device__ __forceinline__ void find_slots(const m3c_cache_params &p, uint32_t first, uint32_t count, int64_t *slots)
+{
+    const uint32_t lane = threadIdx.x % 32u;
+    uint32_t low = 0;                 // sequence `low` begins at or before `first`, or none does
+    uint32_t high = p.sequences;      // `high` does not, or is the end
+    while (high - low > 1u) {
+        const uint32_t step = (high - low + 31u) / 32u;
+        const uint32_t s = low + lane * step;
+        const bool before = s < high && p.offsets[s] <= static_cast<int64_t>(first);
+        const uint32_t begun = __popc(__ballot_sync(0xffffffffu, before));
+        low = begun == 0u ? low : low + (begun - 1u) * step;
+        high = min(low + step, high);
+    }
+    for (uint32_t r = lane; r < count; r += 32u) {
+        uint32_t s = low;
+        while (s + 1u < p.sequences && p.offsets[s + 1u] <= static_cast<int64_t>(first + r)) ++s;
+        slots[r] = slot_in_sequence(p, first + r, s);
+    }
+}
 
+// The vector kernels: vectors of a multiple of eight elements, rows aligned for
+// 16-byte accesses.  `lanes` lanes (a power of two) own a vector, P pieces of
+// eight elements each, piece j of lane l being number j * lanes + l.  A thread
+// keeps its place (keys or values, head, lane) for several rows; blockIdx.y
+// takes over where a row's vectors do not fit a block.  The slots of a CTA's
+// rows are found once, in shared memory.  Bytes bound both directions: three
+// per element of 16-bit rows.
 struct cache_shape {
-    m3c_fastdiv of_row;     // vectors of a row
-    uint32_t vectors;       // of the batch
-    uint32_t lanes;         // of a vector
     uint32_t lane_shift;
+    uint32_t vectors;       // of a row, in a block
+    uint32_t rows;          // side by side in a block
+    uint32_t steps;         // groups of such rows, one after another
 };
 
-template <int DT, bool WRITE>
-__global__ void __launch_bounds__(QUANT_THREADS)
-    cache_kernel(const __grid_constant__ m3c_cache_params p, const __grid_constant__ cache_shape shape)
-{
-    constexpr int DEPTH = WRITE ? CACHE_DEPTH_WRITE : CACHE_DEPTH_READ;
-    __shared__ int64_t slots[CACHE_MOST_ROWS];
-    const uint32_t per_pass = QUANT_THREADS >> shape.lane_shift;
-    const uint32_t first = blockIdx.x * per_pass * DEPTH;
-    const uint32_t first_row = fastdiv(first, shape.of_row);
-    const uint32_t last = min(first + per_pass * DEPTH, shape.vectors) - 1u;
-    const uint32_t rows = fastdiv(last, shape.of_row) - first_row + 1u;
-    const uint32_t element = (threadIdx.x & (shape.lanes - 1u)) * 8u;
-    const bool inside = element < p.head_dim;
-    uint32_t row[DEPTH];
-    uint32_t head[DEPTH];
-    int kv[DEPTH];
-    bool live[DEPTH];
-    uint64_t at[DEPTH];      // the lane's place among the rows' elements
-    Piece<DT, 8> piece[DEPTH];
-#pragma unroll
-    for (int i = 0; i < DEPTH; ++i) {
-        const uint32_t v = first + i * per_pass + (threadIdx.x >> shape.lane_shift);
-        live[i] = v <= last;
-        row[i] = live[i] ? fastdiv(v, shape.of_row) : first_row;
-        const uint32_t rest = live[i] ? v - row[i] * shape.of_row.divisor : 0u;
-        kv[i] = rest >= p.heads ? 1 : 0;
-        head[i] = rest - (kv[i] ? p.heads : 0u);
-        at[i] = row[i] * p.token_stride[kv[i]] + head[i] * p.head_stride[kv[i]] + element;
-        piece[i] = {};
-        if (WRITE && live[i] && inside) piece[i] = load_piece<DT, 8>(p.rows[kv[i]], at[i]);
+constexpr int CACHE_THREADS = 512;    // at most; 256 where the shape allows
+constexpr uint32_t CACHE_STEPS = 8;   // at most
+constexpr uint32_t CACHE_SLOTS = 128 * CACHE_STEPS;  // 256 threads, one head of eight elements
+
+// A thread's place in its block's rows.
+struct cache_place {
+    uint32_t lane;
+    uint32_t lanes;
+    uint32_t side;          // the row's place in the block
+    uint32_t head;
+    int kv;
+    bool owner;             // of a vector at all
+    uint32_t first;         // the block's rows
+    uint32_t count;
+
+    __device__ __forceinline__ cache_place(const m3c_cache_params &p, const cache_shape &shape)
+    {
+        lanes = 1u << shape.lane_shift;
+        lane = threadIdx.x & (lanes - 1u);
+        const uint32_t place = threadIdx.x >> shape.lane_shift;
+        side = place / shape.vectors;
+        const uint32_t vector = blockIdx.y * shape.vectors + place - side * shape.vectors;
+        owner = side < shape.rows && vector < 2u * p.heads;
+        kv = vector >= p.heads ? 1 : 0;
+        head = vector - (kv ? p.heads : 0u);
+        first = blockIdx.x * shape.rows * shape.steps;
+        count = min(shape.rows * shape.steps, p.row_count - first);
     }
-    for (uint32_t r = threadIdx.x; r < rows; r += QUANT_THREADS) slots[r] = cache_slot(p, first_row + r);
+};
+
+// Writing: the CTA walks over its rows, the next rows' loads on their way while
+// one row's codes are made; the slots are found behind the first loads.
+template <int DT, int P>
+__global__ void __launch_bounds__(CACHE_THREADS, 2)
+    cache_write_kernel(const __grid_constant__ m3c_cache_params p, const __grid_constant__ cache_shape shape)
+{
+    __shared__ int64_t slots[CACHE_SLOTS];
+    const cache_place at(p, shape);
+    const uint64_t token_stride = p.token_stride[at.kv];
+    const char *base = static_cast<const char *>(p.rows[at.kv]) +
+                       (at.first * token_stride + at.head * p.head_stride[at.kv] + at.lane * 8u) *
+                           (DT == M3C_F32 ? 4u : 2u);
+    uint8_t *const codes = p.codes[at.kv] + at.lane * 8u;
+    float *const scales = p.scales[at.kv];
+    bool inside[P];
+#pragma unroll
+    for (int j = 0; j < P; ++j) inside[j] = at.owner && (j * at.lanes + at.lane) * 8u < p.head_dim;
+    auto load = [&](uint32_t r, Piece<DT, 8> (&piece)[P]) {
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            piece[j] = {};
+            if (inside[j] && r < at.count) piece[j] = load_piece<DT, 8>(base, r * token_stride + j * at.lanes * 8u);
+        }
+    };
+    Piece<DT, 8> next[P];
+    load(at.side, next);
+    if (threadIdx.x < 32u) find_slots(p, at.first, at.count, slots);
     __syncthreads();
-    if constexpr (WRITE) {
+    // the loop's bounds are the block's, so that its shuffles are whole
+    for (uint32_t r0 = 0; r0 < at.count; r0 += shape.rows) {
+        const uint32_t r = r0 + at.side;
+        float x[P][8];
+        float most = 0.0f;
 #pragma unroll
-        for (int i = 0; i < DEPTH; ++i) {
-            float x[8];
-            widen_piece<DT, 8>(piece[i], x);
-            uint32_t largest = as_bits(largest_of<8>(x));
-            for (uint32_t d = 1; d < shape.lanes; d <<= 1) {
-                const uint32_t other = __shfl_xor_sync(0xffffffffu, largest, d);
-                largest = other > largest ? other : largest;
-            }
-            const int64_t slot = slots[row[i] - first_row];
-            if (!live[i] || slot < 0) continue;
+        for (int j = 0; j < P; ++j) {
+            widen_piece<DT, 8>(next[j], x[j]);
+            const float m = largest_of<8>(x[j]);
+            asm("max.NaN.f32 %0, %1, %2;" : "=f"(most) : "f"(most), "f"(m));
+        }
+        load(r + shape.rows, next);
+        uint32_t largest = as_bits(most);
+        for (uint32_t d = 1; d < at.lanes; d <<= 1) {
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, largest, d);
+            largest = other > largest ? other : largest;
+        }
+        const int64_t slot = at.owner && r < at.count ? slots[r] : -1;
+        if (slot >= 0) {
             const e4m3_divisor d = e4m3_divide_by(e4m3_scale(largest));
-            const uint64_t vector = static_cast<uint64_t>(slot) * p.heads + head[i];
-            if (element == 0u) p.scales[kv[i]][vector] = d.scale;
-            if (inside) e4m3_store<8>(p.codes[kv[i]] + vector * p.head_dim + element, x, d);
-        }
-    } else {
-        uint2 codes[DEPTH];
-        float scale[DEPTH];
+            const uint64_t vector = static_cast<uint64_t>(slot) * p.heads + at.head;
+            if (at.lane == 0u) scales[vector] = d.scale;
 #pragma unroll
-        for (int i = 0; i < DEPTH; ++i) {
-            const int64_t slot = slots[row[i] - first_row];
-            live[i] = live[i] && slot >= 0 && inside;
-            codes[i] = {};
-            scale[i] = 0.0f;
-            if (live[i]) {
-                const uint64_t vector = static_cast<uint64_t>(slot) * p.heads + head[i];
-                codes[i] = __ldcs(reinterpret_cast<const uint2 *>(p.codes[kv[i]] + vector * p.head_dim + element));
-                scale[i] = p.scales[kv[i]][vector];
+            for (int j = 0; j < P; ++j) {
+                if (inside[j]) e4m3_store<8>(codes + vector * p.head_dim + j * at.lanes * 8u, x[j], d);
             }
         }
+    }
+}
+
+// Reading: the slots first, then STEPS rows of a thread at once.
+template <int DT, int P, int STEPS>
+__global__ void __launch_bounds__(CACHE_THREADS)
+    cache_read_kernel(const __grid_constant__ m3c_cache_params p, const __grid_constant__ cache_shape shape)
+{
+    __shared__ int64_t slots[128 * STEPS];
+    const cache_place at(p, shape);
+    if (threadIdx.x < 32u) find_slots(p, at.first, at.count, slots);
+    __syncthreads();
+    if (!at.owner) return;
+    const uint64_t token_stride = p.token_stride[at.kv];
+    char *const base = static_cast<char *>(p.rows[at.kv]) +
+                       (at.first * token_stride + at.head * p.head_stride[at.kv] + at.lane * 8u) *
+                           (DT == M3C_F32 ? 4u : 2u);
+    const uint8_t *const from = p.codes[at.kv] + at.lane * 8u;
+    uint2 codes[STEPS][P];
+    float scale[STEPS];
+    bool live[STEPS];
 #pragma unroll
-        for (int i = 0; i < DEPTH; ++i) {
+    for (int i = 0; i < STEPS; ++i) {
+        const uint32_t r = i * shape.rows + at.side;
+        const int64_t slot = r < at.count ? slots[r] : -1;
+        const uint64_t vector = static_cast<uint64_t>(slot) * p.heads + at.head;
+        live[i] = slot >= 0;
+        scale[i] = live[i] ? p.scales[at.kv][vector] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            codes[i][j] = {};
+            if (live[i] && (j * at.lanes + at.lane) * 8u < p.head_dim) {
+                codes[i][j] = __ldcs(reinterpret_cast<const uint2 *>(from + vector * p.head_dim + j * at.lanes * 8u));
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+        const uint32_t r = i * shape.rows + at.side;
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
             float x[8];
-            e4m3_values(codes[i], x);
+            e4m3_values(codes[i][j], x);
             multiply(x, scale[i]);
-            if (live[i]) store_piece<DT, 8>(p.rows[kv[i]], at[i], narrow_piece<DT>(x));
+            if (live[i] && (j * at.lanes + at.lane) * 8u < p.head_dim) {
+                store_piece<DT, 8, true>(base, r * token_stride + j * at.lanes * 8u, narrow_piece<DT>(x));
+            }
         }
     }
 }
@@ -652,6 +732,7 @@ __global__ void __launch_bounds__(QUANT_THREADS)
 template <bool WRITE>
 __global__ void __launch_bounds__(QUANT_THREADS) cache_any_kernel(const __grid_constant__ m3c_cache_params p)
 {
+    __shared__ int64_t slots[QUANT_WARPS];
     const int lane = static_cast<int>(threadIdx.x) % 32;
     const uint64_t vectors = static_cast<uint64_t>(p.row_count) * 2u * p.heads;
     const uint64_t stride = static_cast<uint64_t>(gridDim.x) * QUANT_WARPS;
@@ -660,8 +741,10 @@ __global__ void __launch_bounds__(QUANT_THREADS) cache_any_kernel(const __grid_c
         const uint32_t rest = static_cast<uint32_t>(v % (2u * p.heads));
         const int kv = rest >= p.heads ? 1 : 0;
         const uint32_t head = rest - kv * p.heads;
-        int64_t slot = lane == 0 ? cache_slot(p, t) : 0;
-        slot = __shfl_sync(0xffffffffu, slot, 0);
+        __syncwarp();
+        find_slots(p, t, 1u, &slots[threadIdx.x / 32]);
+        __syncwarp();
+        const int64_t slot = slots[threadIdx.x / 32];
         if (slot < 0) continue;
         const uint64_t at = static_cast<uint64_t>(slot) * p.heads + head;
         const uint64_t row = t * p.token_stride[kv] + head * p.head_stride[kv];
@@ -686,34 +769,83 @@ __global__ void __launch_bounds__(QUANT_THREADS) cache_any_kernel(const __grid_c
     }
 }
 
-template <int DT, bool WRITE>
-int launch_cache_vectors(const m3c_cache_params &p, const cache_shape &shape, cudaStream_t stream)
+template <int DT, bool WRITE, int P>
+int launch_cache_vectors(const m3c_cache_params &p, cudaStream_t stream)
 {
-    const uint32_t each = (QUANT_THREADS >> shape.lane_shift) * (WRITE ? CACHE_DEPTH_WRITE : CACHE_DEPTH_READ);
-    cache_kernel<DT, WRITE><<<(shape.vectors - 1u) / each + 1u, QUANT_THREADS, 0, stream>>>(p, shape);
+    cache_shape shape;
+    shape.lane_shift = 0u;
+    while ((8u * P << shape.lane_shift) < p.head_dim) ++shape.lane_shift;
+    const uint32_t fit = CACHE_THREADS >> shape.lane_shift;
+    const uint32_t all = 2u * p.heads;
+    shape.vectors = all < fit ? all : fit;
+    const uint32_t threads = shape.vectors << shape.lane_shift;
+    shape.rows = threads < 256u ? 256u / threads : 1u;
+    const uint32_t block = (shape.rows * threads + 31u) / 32u * 32u;
+    const uint32_t chunks = (all - 1u) / shape.vectors + 1u;
+    const uint64_t groups = static_cast<uint64_t>((p.row_count - 1u) / shape.rows + 1u) * chunks;
+    const uint64_t waves = groups / (4u * static_cast<uint64_t>(sm_count()));  // of four CTAs per SM
+    if constexpr (WRITE) {
+        // as many steps as leave every SM its CTAs
+        shape.steps = waves < 1u ? 1u : waves > CACHE_STEPS ? CACHE_STEPS : static_cast<uint32_t>(waves);
+        const dim3 grid((p.row_count - 1u) / (shape.rows * shape.steps) + 1u, chunks);
+        cache_write_kernel<DT, P><<<grid, block, 0, stream>>>(p, shape);
+    } else {
+        // a small batch takes one: the unrolled code's own fetch costs more
+        // than it hides
+        constexpr int MANY = P == 1 ? 4 : 2;
+        shape.steps = waves < MANY ? 1u : MANY;
+        const dim3 grid((p.row_count - 1u) / (shape.rows * shape.steps) + 1u, chunks);
+        if (shape.steps == 1u) {
+            cache_read_kernel<DT, P, 1><<<grid, block, 0, stream>>>(p, shape);
+        } else {
+            cache_read_kernel<DT, P, MANY><<<grid, block, 0, stream>>>(p, shape);
+        }
+    }
     return static_cast<int>(cudaGetLastError());
+}
+
+// The pieces per lane: as few idle lanes as can be (eight elements a piece,
+// lanes a power of two), and of equals the more pieces.
+template <int DT, bool WRITE>
+int launch_cache_pieces(const m3c_cache_params &p, cudaStream_t stream)
+{
+    // four pieces of F32, or of rows held while the next are read, leave too few
+    // threads on an SM
+    constexpr int MOST = WRITE || DT == M3C_F32 ? 3 : 4;
+    const uint32_t pieces = p.head_dim / 8u;
+    int best = 1;
+    uint32_t idle = UINT32_MAX;
+    for (int k = 1; k <= MOST; ++k) {
+        uint32_t lanes = 1u;
+        while (lanes * k < pieces) lanes <<= 1;
+        if (lanes * k - pieces <= idle) {
+            idle = lanes * k - pieces;
+            best = k;
+        }
+    }
+    switch (best) {
+    case 1: return launch_cache_vectors<DT, WRITE, 1>(p, stream);
+    case 2: return launch_cache_vectors<DT, WRITE, 2>(p, stream);
+    case 3: return launch_cache_vectors<DT, WRITE, 3>(p, stream);
+    default: return launch_cache_vectors<DT, WRITE, MOST>(p, stream);
+    }
 }
 
 template <bool WRITE>
 int launch_cache(const m3c_cache_params &p, cudaStream_t stream)
 {
     const uint64_t vectors = static_cast<uint64_t>(p.row_count) * 2u * p.heads;
-    const uint64_t step = p.dtype[0] == M3C_F32 ? 4u : 8u;  // elements of 16 bytes
-    bool fits = p.dtype[0] == p.dtype[1] && p.head_dim % 8u == 0u && p.head_dim <= 256u && vectors < (1ull << 31);
+    // a vector's lanes are at most a warp; the grid's y counts heads
+    bool fits = p.dtype[0] == p.dtype[1] && p.head_dim % 8u == 0u && p.head_dim <= 256u && p.heads <= 16384u;
     for (int k = 0; k < 2; ++k) {
-        fits = fits && aligned_to(p.rows[k], 16) && p.token_stride[k] % step == 0u && p.head_stride[k] % step == 0u;
+        fits = fits && aligned_to(p.rows[k], p.dtype[0] == M3C_F32 ? 32 : 16) && p.token_stride[k] % 8u == 0u &&
+               p.head_stride[k] % 8u == 0u;
     }
     if (fits) {
-        cache_shape shape;
-        m3c_fastdiv_init(&shape.of_row, 2u * p.heads);
-        shape.vectors = static_cast<uint32_t>(vectors);
-        shape.lane_shift = 0u;
-        while ((8u << shape.lane_shift) < p.head_dim) ++shape.lane_shift;
-        shape.lanes = 1u << shape.lane_shift;
         switch (p.dtype[0]) {
-        case M3C_F16: return launch_cache_vectors<M3C_F16, WRITE>(p, shape, stream);
-        case M3C_BF16: return launch_cache_vectors<M3C_BF16, WRITE>(p, shape, stream);
-        default: return launch_cache_vectors<M3C_F32, WRITE>(p, shape, stream);
+        case M3C_F16: return launch_cache_pieces<M3C_F16, WRITE>(p, stream);
+        case M3C_BF16: return launch_cache_pieces<M3C_BF16, WRITE>(p, stream);
+        default: return launch_cache_pieces<M3C_F32, WRITE>(p, stream);
         }
     }
     const unsigned grid = capped_grid((vectors + QUANT_WARPS - 1) / QUANT_WARPS, 32u);
