@@ -15,9 +15,7 @@ namespace {
 
 constexpr int QUANT_THREADS = 256;
 constexpr int QUANT_WARPS = QUANT_THREADS / 32;
-#ifndef NORM_THREADS
-#define NORM_THREADS 128
-#endif
+constexpr int NORM_THREADS = 128;                   // rows share a CTA up to these
 constexpr uint64_t NORM_WIDEST = 16384;             // of the register kernel
 constexpr uint64_t NORM_KEPT_BYTES = 200u * 1024u;  // of shared memory for a row
 
