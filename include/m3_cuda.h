@@ -17,8 +17,10 @@
  *     (src/m3_provider.c) can register this library as one more provider.
  *
  *  3. CUDA-only extensions: device and stream selection, asynchronous runs,
- *     device pointers of session values, a host-only planner for tests, and
- *     the seeded input generators of the reference's m3_rng.
+ *     device pointers of session values, a host-only planner for tests, the
+ *     seeded input generators of the reference's m3_rng, and stream-ordered
+ *     operators of a served language model (RMS norm into 8 bits, a paged
+ *     8-bit key/value cache, verification of drafted tokens).
  *
  * ABI compatibility.  The reference types that cross this boundary are
  * restated below with identical layout.  Each block is guarded by the
@@ -28,7 +30,8 @@
  *
  * Operators executed on the GPU: COPY, CAST, ADD, MUL, GATED_SILU, SOFTMAX,
  * TOP_K, CATEGORICAL, RMS_NORM, LAYER_NORM, SNAKE1D, TANH, and the extensions
- * M3_OP_ABS_MAX and M3_OP_CLAMP_UNIT.  Other m3.h kinds (contractions,
+ * M3_OP_ABS_MAX, M3_OP_CLAMP_UNIT, M3_OP_ROW_SUM, M3_OP_RMS_NORM_E4M3 and
+ * M3_OP_VERIFY_DRAFT.  Other m3.h kinds (contractions,
  * attention, convolutions, embedding, RoPE) are rejected with
  * M3_STATUS_UNSUPPORTED at session creation; there is no CPU fallback inside
  * this library.
@@ -448,6 +451,34 @@ typedef struct {
  * graph shares one row pass. */
 #define M3_OP_ROW_SUM ((m3_op_kind)66)
 
+/* Extension dtype: one byte, one sign, four exponent and three significand
+ * bits, largest value 448, no infinity, 0x7f and 0xff are NaN.  Only
+ * M3_OP_RMS_NORM_E4M3 makes values of it; no other operator takes it. */
+#define M3_DTYPE_E4M3 ((m3_dtype)64)
+
+/* M3_OP_RMS_NORM_E4M3 (extension, session only): the RMS norm into 8 bits, as
+ * m3_cuda_rms_norm_e4m3 below computes it.  inputs[0] [..., width], inputs[1]
+ * the norm's weight [width] (each F32, F16 or BF16), parameters.norm.epsilon;
+ * outputs[0] the codes, M3_DTYPE_E4M3 of the input's shape, outputs[1] their
+ * scales, F32 [..., groups], where `groups` divides width: each width / groups
+ * consecutive elements share a scale (an inferred outputs[1] has one group).
+ * An ADD of equal shapes and dtypes that feeds it runs in the same launch.
+ *
+ * M3_OP_VERIFY_DRAFT (extension, session only): the verification of drafted
+ * tokens, as m3_cuda_verify_draft below computes it.  inputs[0] the target's
+ * probabilities [batch, drafts + 1, vocabulary], inputs[1] the drafted tokens
+ * I32 [batch, drafts], inputs[2] uniforms F32 [batch, drafts + 1], inputs[3]
+ * (optional) the draft model's probabilities [batch, drafts, vocabulary] of
+ * inputs[0]'s dtype, inputs[4] (optional) lengths I32 [batch]; outputs[0] the
+ * tokens I32 [batch, drafts + 1], outputs[1] the accepted counts I32 [batch].
+ * It has no data check: a bad sequence is reported in its own place, so it
+ * does not fail the run of its batch.
+ *
+ * Session only: the backend plug-in's command type has no descriptors for
+ * these two; m3_cuda_backend_supports_kind is false for them. */
+#define M3_OP_RMS_NORM_E4M3 ((m3_op_kind)67)
+#define M3_OP_VERIFY_DRAFT ((m3_op_kind)68)
+
 #define M3_CUDA_DEVICE_CURRENT (-1)
 
 typedef struct {
@@ -607,8 +638,8 @@ m3_status m3_cuda_graph_plan(const m3_graph *graph,
  * extent allows); a value of extent 1 there, or without that axis, is
  * replicated (broadcast constants such as a snake alpha [1,C,1] split along
  * time, a norm scale, scalars).  Row operators (SOFTMAX, TOP_K, ROW_SUM,
- * RMS_NORM, LAYER_NORM, CATEGORICAL) need the split axis to differ from
- * their input's last axis.  M3_OP_ABS_MAX is a global reduction: every rank
+ * RMS_NORM, RMS_NORM_E4M3, LAYER_NORM) need the split axis to differ from
+ * their input's last axis; CATEGORICAL and VERIFY_DRAFT are not split.  M3_OP_ABS_MAX is a global reduction: every rank
  * reduces its slab, then one NCCL all-reduce (MAX over the unsigned bit
  * patterns, exact and order-free) on the session's stream gives every rank
  * the global result; its output may not feed another node.  When the graph
@@ -885,7 +916,8 @@ m3_status m3_cuda_abs_max_static(int device, void *stream, m3_dtype dtype,
  * No counterpart in the reference.  A graph's shapes are fixed when its
  * session is created; the rows, sequences and drafts of a serving step change
  * with every step.  These calls therefore take device addresses and sizes,
- * like m3_cuda_abs_max_static, and are stream-ordered: they check their
+ * like m3_cuda_abs_max_static (two of them are graph operators too:
+ * M3_OP_RMS_NORM_E4M3 and M3_OP_VERIFY_DRAFT), and are stream-ordered: they check their
  * arguments on the host, enqueue on `stream` (a cudaStream_t of the device;
  * NULL is the legacy default stream) and return without waiting.  They
  * allocate nothing and may be captured into a CUDA graph.  The calling

@@ -56,7 +56,7 @@ static m3_status fail_cuda(m3_error *error, cudaError_t code, const char *what)
 
 bool m3_cuda_backend_supports_kind(m3_op_kind kind)
 {
-    return m3c_kind_supported(kind);
+    return m3c_kind_supported(kind) && !m3c_kind_session_only(kind);
 }
 
 m3_status m3_cuda_backend_context_create(
@@ -1191,6 +1191,11 @@ m3_status m3_cuda_backend_execute(void *context, const m3_command *commands,
     for (i = 0U; i < command_count; ++i) {
         m3c_vcommand v;
 
+        if (m3c_kind_session_only(commands[i].kind)) {
+            return m3c_error_set(error, M3_STATUS_UNSUPPORTED,
+                                 "unsupported operation kind %d",
+                                 (int)commands[i].kind);
+        }
         to_vcommand(&commands[i], &v);
         status = m3c_validate(&v, error);
         if (status != M3_STATUS_OK) {

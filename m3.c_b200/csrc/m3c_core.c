@@ -88,6 +88,9 @@ m3_status m3c_error_set(m3_error *error, m3_status status, const char *format,
 
 size_t m3c_dtype_size(m3_dtype dtype)
 {
+    if (dtype == M3_DTYPE_E4M3) {
+        return 1U;
+    }
     return (dtype == M3_DTYPE_F16 || dtype == M3_DTYPE_BF16) ? 2U : 4U;
 }
 
@@ -98,7 +101,7 @@ bool m3c_dtype_float(m3_dtype dtype)
 }
 
 /* Same contract and statuses as the reference's m3_tensor_metadata_init
- * (src/m3_tensor.c:39-102): a known dtype, rank <= 8, element and byte counts
+ * (src/m3_tensor.c:39-102): a known dtype (or the extension E4M3), rank <= 8, element and byte counts
  * without overflow. */
 m3_status m3c_metadata_init(m3_tensor_metadata *metadata, m3_dtype dtype,
                             uint8_t rank, const uint64_t *shape,
@@ -111,7 +114,8 @@ m3_status m3c_metadata_init(m3_tensor_metadata *metadata, m3_dtype dtype,
         return m3c_error_set(error, M3_STATUS_INVALID_ARGUMENT,
                              "tensor metadata output is null");
     }
-    if ((int)dtype < (int)M3_DTYPE_F32 || (int)dtype > (int)M3_DTYPE_I32) {
+    if (((int)dtype < (int)M3_DTYPE_F32 || (int)dtype > (int)M3_DTYPE_I32) &&
+        dtype != M3_DTYPE_E4M3) {
         return m3c_error_set(error, M3_STATUS_UNSUPPORTED,
                              "unsupported tensor dtype value %d", (int)dtype);
     }

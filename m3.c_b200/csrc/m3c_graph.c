@@ -263,7 +263,9 @@ static m3_status infer_shape(const m3_graph *graph,
     if (status != M3_STATUS_OK) {
         return status;
     }
-    if (output_index != 0U && node->kind != M3_OP_TOP_K) {
+    if (output_index != 0U && node->kind != M3_OP_TOP_K &&
+        !(output_index == 1U && (node->kind == M3_OP_RMS_NORM_E4M3 ||
+                                 node->kind == M3_OP_VERIFY_DRAFT))) {
         return m3c_error_set(error, M3_STATUS_OUT_OF_RANGE,
                              "operation has no requested inferred output");
     }
@@ -298,6 +300,30 @@ static m3_status infer_shape(const m3_graph *graph,
         copy_shape(out, first);
         out->shape[first->rank - 1U] = 1U;
         out->dtype = M3_DTYPE_F32;
+        return M3_STATUS_OK;
+    case (int)M3_OP_RMS_NORM_E4M3:
+        if (first->rank == 0U) {
+            return m3c_error_set(error, M3_STATUS_INVALID_ARGUMENT,
+                                 "cannot infer norm shape");
+        }
+        copy_shape(out, first);
+        out->dtype = M3_DTYPE_E4M3;
+        if (output_index == 1U) {
+            out->shape[first->rank - 1U] = 1U;
+            out->dtype = M3_DTYPE_F32;
+        }
+        return M3_STATUS_OK;
+    case (int)M3_OP_VERIFY_DRAFT:
+        if (first->rank != 3U) {
+            return m3c_error_set(error, M3_STATUS_INVALID_ARGUMENT,
+                                 "cannot infer verification shape");
+        }
+        out->rank = output_index == 0U ? 2U : 1U;
+        out->shape[0] = first->shape[0];
+        if (output_index == 0U) {
+            out->shape[1] = first->shape[1];
+        }
+        out->dtype = M3_DTYPE_I32;
         return M3_STATUS_OK;
     case M3_OP_ADD:
     case M3_OP_MUL:

@@ -67,14 +67,16 @@ typedef struct {
 /* One operator with its views, in reference positions. */
 typedef struct {
     m3_op_kind kind;
-    m3c_vview in[3];
-    m3c_vview out[2];
+    m3c_vview in[M3_GRAPH_NODE_INPUT_CAPACITY];
+    m3c_vview out[M3_GRAPH_NODE_OUTPUT_CAPACITY];
     float epsilon;
     uint64_t k;
 } m3c_vcommand;
 
 m3_status m3c_validate(const m3c_vcommand *command, m3_error *error);
 bool m3c_kind_supported(m3_op_kind kind);
+/* Operators of the graph API that the backend plug-in has no command for. */
+bool m3c_kind_session_only(m3_op_kind kind);
 const char *m3c_kind_name(m3_op_kind kind);
 
 /* ---------------------------------------------------------------- plan */
@@ -83,8 +85,12 @@ typedef enum {
     M3C_LAUNCH_EW = 0,
     M3C_LAUNCH_SOFTMAX,     /* softmax, top-k and/or row sums of the same rows */
     M3C_LAUNCH_NORM,        /* RMSNorm / LayerNorm, optional residual add */
-    M3C_LAUNCH_CATEGORICAL  /* categorical sampling: row_in probabilities,
+    M3C_LAUNCH_CATEGORICAL, /* categorical sampling: row_in probabilities,
                                row_in_b uniforms, row_out indices */
+    M3C_LAUNCH_NORM_E4M3,   /* RMSNorm into row_out codes and row_out2 scales,
+                               optional residual add */
+    M3C_LAUNCH_VERIFY       /* draft verification: node_in[0..4] as the node's
+                               inputs, row_out tokens, row_out2 accepted */
 } m3c_launch_kind;
 
 /* A reference to a value's device bytes at run time: slot + byte offset, and
@@ -128,6 +134,7 @@ typedef struct {
     m3c_ref row_out4;              /* row sums */
     m3c_ref norm_scale;
     m3c_ref norm_bias;
+    m3c_ref node_in[M3_GRAPH_NODE_INPUT_CAPACITY];
     bool layer_norm;
     float epsilon;
     uint64_t k;

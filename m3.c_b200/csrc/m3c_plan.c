@@ -83,6 +83,15 @@ static m3_status regular_schema(m3_op_kind kind, schema_t *schema,
         schema->inputs = 1U;
         schema->outputs = 2U;
         return M3_STATUS_OK;
+    case (int)M3_OP_RMS_NORM_E4M3:
+        schema->inputs = 2U;
+        schema->outputs = 2U;
+        return M3_STATUS_OK;
+    case (int)M3_OP_VERIFY_DRAFT:
+        schema->inputs = 5U;
+        schema->outputs = 2U;
+        schema->optional = (1U << 3U) | (1U << 4U);
+        return M3_STATUS_OK;
     default:
         return m3c_error_set(error, M3_STATUS_UNSUPPORTED,
                              "unsupported graph operation kind %d",
@@ -329,17 +338,21 @@ static m3_status validate_node(const m3_graph *graph, const m3c_plan *plan,
                                const m3_graph_node_desc *node,
                                m3_error *error)
 {
-    size_t strides[5][M3_TENSOR_MAX_RANK];
+    enum {
+        INPUTS = M3_GRAPH_NODE_INPUT_CAPACITY,
+        OUTPUTS = M3_GRAPH_NODE_OUTPUT_CAPACITY
+    };
+    size_t strides[INPUTS + OUTPUTS][M3_TENSOR_MAX_RANK];
     m3c_vcommand command;
     int i;
 
     memset(&command, 0, sizeof(command));
     command.kind = node->kind;
-    for (i = 0; i < 3; ++i) {
+    for (i = 0; i < INPUTS; ++i) {
         value_view(graph, plan, node->inputs[i], strides[i], &command.in[i]);
     }
-    for (i = 0; i < 2; ++i) {
-        value_view(graph, plan, node->outputs[i], strides[3 + i],
+    for (i = 0; i < OUTPUTS; ++i) {
+        value_view(graph, plan, node->outputs[i], strides[INPUTS + i],
                    &command.out[i]);
     }
     command.epsilon = node->parameters.norm.epsilon;
@@ -1173,6 +1186,36 @@ static m3_status plan_categorical(planner *p, size_t n, m3_error *error)
     return status;
 }
 
+/* Row launch for draft verification.  A bad sequence is reported in its own
+ * outputs, so the launch cannot fail and writes them in place. */
+static m3_status plan_verify(planner *p, size_t n, m3_error *error)
+{
+    const m3_graph_node_desc *node = &p->graph->nodes[n];
+    m3c_launch launch;
+    m3_status status;
+    size_t i;
+
+    memset(&launch, 0, sizeof(launch));
+    launch.kind = M3C_LAUNCH_VERIFY;
+    launch.first_node = n;
+    launch.node_count = 1U;
+    for (i = 0U; i < M3_GRAPH_NODE_INPUT_CAPACITY; ++i) {
+        launch.node_in[i].value = NO_VALUE;
+        if (node->inputs[i] != M3_GRAPH_VALUE_NONE) {
+            launch.node_in[i] = read_ref(p, node->inputs[i]);
+        }
+    }
+    launch.command_a = (uint32_t)n;
+    status = write_ref(p, node->outputs[0], false, (uint32_t)n,
+                       &launch.row_out, error);
+    if (status == M3_STATUS_OK) {
+        status = write_ref(p, node->outputs[1], false, (uint32_t)n,
+                           &launch.row_out2, error);
+    }
+    (void)snprintf(launch.text, sizeof(launch.text), "row[VERIFY_DRAFT]");
+    return status == M3_STATUS_OK ? push_launch(p, &launch, error) : status;
+}
+
 /* Row launch for a norm; `residual` is the index of an ADD node whose output
  * is the norm input and that runs as the kernel's prologue (or SIZE_MAX). */
 static m3_status plan_norm(planner *p, size_t n, size_t residual,
@@ -1183,7 +1226,8 @@ static m3_status plan_norm(planner *p, size_t n, size_t residual,
     m3_status status = M3_STATUS_OK;
 
     memset(&launch, 0, sizeof(launch));
-    launch.kind = M3C_LAUNCH_NORM;
+    launch.kind = node->kind == M3_OP_RMS_NORM_E4M3 ? M3C_LAUNCH_NORM_E4M3
+                                                    : M3C_LAUNCH_NORM;
     launch.first_node = residual != SIZE_MAX ? residual : n;
     launch.node_count = residual != SIZE_MAX ? 2U : 1U;
     launch.layer_norm = node->kind == M3_OP_LAYER_NORM;
@@ -1221,9 +1265,13 @@ static m3_status plan_norm(planner *p, size_t n, size_t residual,
         status = write_ref(p, node->outputs[0], false, (uint32_t)n,
                            &launch.row_out, error);
     }
+    if (status == M3_STATUS_OK && launch.kind == M3C_LAUNCH_NORM_E4M3) {
+        status = write_ref(p, node->outputs[1], false, (uint32_t)n,
+                           &launch.row_out2, error);
+    }
     (void)snprintf(launch.text, sizeof(launch.text), "row[%s%s]",
                    residual != SIZE_MAX ? "ADD+" : "",
-                   launch.layer_norm ? "LAYER_NORM" : "RMS_NORM");
+                   m3c_kind_name(node->kind));
     return status == M3_STATUS_OK ? push_launch(p, &launch, error) : status;
 }
 
@@ -1268,6 +1316,13 @@ static bool residual_prologue(const planner *p, const node_list *open,
 
         if (sa == ss || sb == ss || sa == so || sb == so) {
             return false;
+        }
+        if (norm->kind == M3_OP_RMS_NORM_E4M3) {
+            size_t s2 = p->plan->value_slot[norm->outputs[1]];
+
+            if (sa == s2 || sb == s2) {
+                return false;
+            }
         }
     }
     return true;
@@ -1314,7 +1369,8 @@ static m3_status fuse(planner *p, bool fuse_enabled, m3_error *error)
             ++n;
             continue;
         }
-        if (node->kind == M3_OP_RMS_NORM || node->kind == M3_OP_LAYER_NORM) {
+        if (node->kind == M3_OP_RMS_NORM || node->kind == M3_OP_LAYER_NORM ||
+            node->kind == M3_OP_RMS_NORM_E4M3) {
             if (fuse_enabled && residual_prologue(p, &open, n)) {
                 size_t add = open.nodes[0];
 
@@ -1335,6 +1391,11 @@ static m3_status fuse(planner *p, bool fuse_enabled, m3_error *error)
         }
         if (node->kind == M3_OP_CATEGORICAL) {
             status = plan_categorical(p, n, error);
+            ++n;
+            continue;
+        }
+        if (node->kind == M3_OP_VERIFY_DRAFT) {
+            status = plan_verify(p, n, error);
             ++n;
             continue;
         }
@@ -1436,8 +1497,18 @@ static m3_status mark_needed_slots(const m3_graph *graph, m3c_plan *plan,
             }
             continue;
         }
-        mark_ref(plan, launch->row_in);
         mark_ref(plan, launch->row_out);
+        if (launch->kind == M3C_LAUNCH_VERIFY) {
+            for (k = 0; k < (int)M3_GRAPH_NODE_INPUT_CAPACITY; ++k) {
+                mark_ref(plan, launch->node_in[k]);
+            }
+            mark_ref(plan, launch->row_out2);
+            continue;
+        }
+        mark_ref(plan, launch->row_in);
+        if (launch->kind == M3C_LAUNCH_NORM_E4M3) {
+            mark_ref(plan, launch->row_out2);
+        }
         if (launch->kind == M3C_LAUNCH_CATEGORICAL) {
             mark_ref(plan, launch->row_in_b);
         } else if (launch->kind == M3C_LAUNCH_SOFTMAX) {

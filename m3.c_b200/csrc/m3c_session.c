@@ -361,6 +361,10 @@ static size_t launch_slots(const m3c_plan *plan, const m3c_launch *l,
         for (k = 0; k < l->n_operands; ++k) refs[n++] = l->operands[k].ref;
         for (k = 0; k < l->n_outputs; ++k) refs[n++] = l->outputs[k];
         if (l->has_absmax) refs[n++] = l->absmax_out;
+    } else if (l->kind == M3C_LAUNCH_VERIFY) {
+        for (k = 0; k < (int)M3_GRAPH_NODE_INPUT_CAPACITY; ++k) refs[n++] = l->node_in[k];
+        refs[n++] = l->row_out;
+        refs[n++] = l->row_out2;
     } else {
         refs[n++] = l->row_in;
         refs[n++] = l->row_in_b;
@@ -746,6 +750,55 @@ static int launch_one(m3_session *s, size_t index, bool first, cudaStream_t stre
             }
         }
         return m3c_launch_softmax(&p, stream);
+    }
+    if (l->kind == M3C_LAUNCH_NORM_E4M3) {
+        const m3_tensor_metadata *in = &s->metadata[l->row_in.value];
+        const m3_tensor_metadata *scales = &s->metadata[l->row_out2.value];
+        m3c_norm_e4m3_params p;
+
+        memset(&p, 0, sizeof(p));
+        p.x = ref_pointer(s, l->row_in);
+        p.resid_b = ref_pointer(s, l->row_in_b);
+        p.sum_out = ref_pointer(s, l->row_sum_out);
+        p.width = in->shape[in->rank - 1U];
+        p.rows = in->element_count / p.width;
+        p.x_stride = p.width;
+        p.resid_stride = p.width;
+        p.sum_stride = p.width;
+        p.scale = ref_pointer(s, l->norm_scale);
+        p.codes = ref_pointer(s, l->row_out);
+        p.code_scales = (float *)ref_pointer(s, l->row_out2);
+        p.group = p.width / scales->shape[scales->rank - 1U];
+        p.dtype = (int32_t)in->dtype;
+        p.scale_dtype = (int32_t)s->metadata[l->norm_scale.value].dtype;
+        p.epsilon = l->epsilon;
+        p.skip_before = (uint32_t)l->first_node;
+        p.status = s->status_device;
+        p.first_of_run = first ? 1 : 0;
+        return m3c_launch_norm_e4m3(&p, stream);
+    }
+    if (l->kind == M3C_LAUNCH_VERIFY) {
+        const m3_tensor_metadata *target = &s->metadata[l->node_in[0].value];
+        m3c_verify_params p;
+
+        memset(&p, 0, sizeof(p));
+        p.target = ref_pointer(s, l->node_in[0]);
+        p.draft_tokens = (const int32_t *)ref_pointer(s, l->node_in[1]);
+        p.uniforms = (const float *)ref_pointer(s, l->node_in[2]);
+        p.draft = ref_pointer(s, l->node_in[3]);
+        p.lengths = (const int32_t *)ref_pointer(s, l->node_in[4]);
+        p.tokens = (int32_t *)ref_pointer(s, l->row_out);
+        p.accepted = (int32_t *)ref_pointer(s, l->row_out2);
+        p.batch = target->shape[0];
+        p.drafts = target->shape[1] - 1U;
+        p.vocabulary = (uint32_t)target->shape[2];
+        p.target_stride = p.vocabulary;
+        p.draft_stride = p.vocabulary;
+        p.dtype = (int32_t)target->dtype;
+        p.status = s->status_device;
+        p.skip_before = (uint32_t)l->first_node;
+        p.first_of_run = first ? 1 : 0;
+        return m3c_launch_verify(&p, stream);
     }
     {
         const m3_tensor_metadata *in = &s->metadata[l->row_in.value];

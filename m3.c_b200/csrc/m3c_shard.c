@@ -12,8 +12,8 @@
  * split axis; their per-row outputs keep the input's rank and split with it.
  * ABS_MAX reduces everything: its one-element output is replicated and
  * combined across ranks after each run (m3c_session.c), so it may not feed
- * another node.  CATEGORICAL drops an axis of its input, which right
- * alignment cannot place, and is not sharded.
+ * another node.  CATEGORICAL and VERIFY_DRAFT drop an axis of their input,
+ * which right alignment cannot place, and are not sharded.
  *
  * Slabs are balanced: in whole blocks of 4 elements when the extent is a
  * multiple of 4 and at least 4 per rank (so vectorised kernels keep full
@@ -64,6 +64,7 @@ static bool row_reducing(m3_op_kind kind)
     case M3_OP_RMS_NORM:
     case M3_OP_LAYER_NORM:
     case (int)M3_OP_ROW_SUM:
+    case (int)M3_OP_RMS_NORM_E4M3:
         return true;
     default:
         return false;
@@ -149,8 +150,10 @@ static bool axis_allowed(const m3_graph *graph, size_t primary, int axis,
     for (n = 0U; n < graph->node_count; ++n) {
         const m3_graph_node_desc *node = &graph->nodes[n];
 
-        if (node->kind == M3_OP_CATEGORICAL) {
-            snprintf(why, why_size, "CATEGORICAL (node %zu) cannot be sharded", n);
+        if (node->kind == M3_OP_CATEGORICAL ||
+            node->kind == M3_OP_VERIFY_DRAFT) {
+            snprintf(why, why_size, "%s (node %zu) cannot be sharded",
+                     m3c_kind_name(node->kind), n);
             return false;
         }
         if (row_reducing(node->kind) && node->inputs[0] < graph->value_count) {

@@ -3,7 +3,7 @@
  * The same checks, order and messages as the reference validators for the
  * operators this provider runs (src/m3_op_validate.c:53-233,
  * src/m3_op_validate_basic.c:5-289, src/m3_op_validate_nn.c:120-164,
- * src/m3_op_validate_sampling.c:13-76), plus the two extension operators.
+ * src/m3_op_validate_sampling.c:13-76), plus the extension operators.
  * Views are abstracted as (metadata, byte offset, byte strides, storage key)
  * so the graph planner and the backend plug-in share one implementation. */
 
@@ -204,6 +204,11 @@ static m3_status validate_copy_cast(const m3c_vcommand *c, m3_error *error)
 
     if (status != M3_STATUS_OK) {
         return status;
+    }
+    if (c->in[0].metadata->dtype == M3_DTYPE_E4M3 ||
+        c->out[0].metadata->dtype == M3_DTYPE_E4M3) {
+        return m3c_error_set(error, M3_STATUS_UNSUPPORTED,
+                             "copy and cast do not take E4M3 tensors");
     }
     if (c->kind == M3_OP_COPY) {
         if (c->in[0].metadata->dtype != c->out[0].metadata->dtype) {
@@ -551,6 +556,145 @@ static m3_status validate_row_sum(const m3c_vcommand *c, m3_error *error)
     return check_alias(&c->out[0], &c->in[0], false, "row-sum", error);
 }
 
+/* Extension: RMS norm into E4M3 codes (out[0]) and F32 scales (out[1]). */
+static m3_status validate_norm_e4m3(const m3c_vcommand *c, m3_error *error)
+{
+    const m3_tensor_metadata *in;
+    const m3_tensor_metadata *scale;
+    const m3_tensor_metadata *scales;
+    uint64_t width;
+    uint64_t groups;
+    uint8_t axis;
+    bool shape_ok;
+    int k;
+    m3_status status = nn_view(&c->in[0], false, "RMSNorm input", error);
+
+    if (status == M3_STATUS_OK) {
+        status = nn_view(&c->in[1], false, "norm scale", error);
+    }
+    if (status == M3_STATUS_OK) {
+        status = check_view(&c->out[0], true, "norm codes", error);
+    }
+    if (status == M3_STATUS_OK) {
+        status = check_view(&c->out[1], true, "norm code scales", error);
+    }
+    if (status != M3_STATUS_OK) {
+        return status;
+    }
+    in = c->in[0].metadata;
+    scale = c->in[1].metadata;
+    scales = c->out[1].metadata;
+    if (c->out[0].metadata->dtype != M3_DTYPE_E4M3 ||
+        scales->dtype != M3_DTYPE_F32) {
+        return m3c_error_set(error, M3_STATUS_INVALID_ARGUMENT,
+                             "norm codes must be E4M3 and their scales F32");
+    }
+    if (in->rank == 0U || !m3c_shape_equal(in, c->out[0].metadata) ||
+        !isfinite(c->epsilon) || c->epsilon <= 0.0F) {
+        return m3c_error_set(error, M3_STATUS_INVALID_ARGUMENT,
+                             "norm shape or epsilon is invalid");
+    }
+    width = in->shape[in->rank - 1U];
+    if (width == 0U || width > (uint64_t)INT32_MAX || scale->rank != 1U ||
+        scale->shape[0] != width) {
+        return m3c_error_set(error, M3_STATUS_INVALID_ARGUMENT,
+                             "norm channel shape is invalid");
+    }
+    shape_ok = scales->rank == in->rank;
+    for (axis = 0U; shape_ok && axis + 1U < in->rank; ++axis) {
+        shape_ok = scales->shape[axis] == in->shape[axis];
+    }
+    groups = shape_ok ? scales->shape[in->rank - 1U] : 0U;
+    if (groups == 0U || width % groups != 0U) {
+        return m3c_error_set(error, M3_STATUS_INVALID_ARGUMENT,
+                             "norm code scales must be [..., groups] with "
+                             "groups dividing the channels");
+    }
+    for (k = 0; status == M3_STATUS_OK && k < 2; ++k) {
+        const char *name = k == 0 ? "norm codes" : "norm code scales";
+
+        status = check_alias(&c->out[k], &c->in[0], false, name, error);
+        if (status == M3_STATUS_OK) {
+            status = check_alias(&c->out[k], &c->in[1], false, name, error);
+        }
+    }
+    if (status == M3_STATUS_OK) {
+        status = check_disjoint(&c->out[0], &c->out[1], "norm", error);
+    }
+    return status;
+}
+
+/* Extension: verification of drafted tokens. */
+static m3_status validate_verify(const m3c_vcommand *c, m3_error *error)
+{
+    static const char *const names[5] = {
+        "target probabilities", "drafted tokens", "verification uniforms",
+        "draft probabilities", "draft lengths"};
+    static const char *const outputs[2] = {"verified tokens",
+                                           "accepted counts"};
+    const m3_tensor_metadata *m[5] = {NULL, NULL, NULL, NULL, NULL};
+    const m3_tensor_metadata *tokens;
+    const m3_tensor_metadata *accepted;
+    uint64_t batch;
+    uint64_t places;
+    uint64_t vocabulary;
+    m3_status status = M3_STATUS_OK;
+    int k;
+    int i;
+
+    for (k = 0; status == M3_STATUS_OK && k < 5; ++k) {
+        if (k < 3 || c->in[k].present) {
+            status = check_view(&c->in[k], false, names[k], error);
+            m[k] = c->in[k].metadata;
+        }
+    }
+    for (k = 0; status == M3_STATUS_OK && k < 2; ++k) {
+        status = check_view(&c->out[k], true, outputs[k], error);
+    }
+    if (status != M3_STATUS_OK) {
+        return status;
+    }
+    tokens = c->out[0].metadata;
+    accepted = c->out[1].metadata;
+    if (!m3c_dtype_float(m[0]->dtype) || m[1]->dtype != M3_DTYPE_I32 ||
+        m[2]->dtype != M3_DTYPE_F32 ||
+        (m[3] != NULL && m[3]->dtype != m[0]->dtype) ||
+        (m[4] != NULL && m[4]->dtype != M3_DTYPE_I32) ||
+        tokens->dtype != M3_DTYPE_I32 || accepted->dtype != M3_DTYPE_I32) {
+        return m3c_error_set(error, M3_STATUS_INVALID_ARGUMENT,
+                             "verification dtype is invalid");
+    }
+    batch = m[0]->rank == 3U ? m[0]->shape[0] : 0U;
+    places = m[0]->rank == 3U ? m[0]->shape[1] : 0U;
+    vocabulary = m[0]->rank == 3U ? m[0]->shape[2] : 0U;
+    if (places == 0U || vocabulary == 0U || vocabulary > (uint64_t)INT32_MAX ||
+        batch > (uint64_t)INT32_MAX || places > (uint64_t)INT32_MAX ||
+        m[1]->rank != 2U || m[1]->shape[0] != batch ||
+        m[1]->shape[1] != places - 1U || m[2]->rank != 2U ||
+        m[2]->shape[0] != batch || m[2]->shape[1] != places ||
+        (m[3] != NULL &&
+         (m[3]->rank != 3U || m[3]->shape[0] != batch ||
+          m[3]->shape[1] != places - 1U || m[3]->shape[2] != vocabulary)) ||
+        (m[4] != NULL && (m[4]->rank != 1U || m[4]->shape[0] != batch)) ||
+        !m3c_shape_equal(tokens, m[2]) || accepted->rank != 1U ||
+        accepted->shape[0] != batch) {
+        return m3c_error_set(error, M3_STATUS_INVALID_ARGUMENT,
+                             "verification shape is invalid");
+    }
+    for (k = 0; status == M3_STATUS_OK && k < 2; ++k) {
+        for (i = 0; status == M3_STATUS_OK && i < 5; ++i) {
+            if (m[i] != NULL) {
+                status = check_alias(&c->out[k], &c->in[i], false, outputs[k],
+                                     error);
+            }
+        }
+    }
+    if (status == M3_STATUS_OK) {
+        status = check_disjoint(&c->out[0], &c->out[1], "verification", error);
+    }
+    return status;
+}
+
 /* Extension: bit-preserving clamp of F32 to [-1, 1]. */
 static m3_status validate_clamp(const m3c_vcommand *c, m3_error *error)
 {
@@ -586,10 +730,17 @@ bool m3c_kind_supported(m3_op_kind kind)
     case (int)M3_OP_ABS_MAX:
     case (int)M3_OP_CLAMP_UNIT:
     case (int)M3_OP_ROW_SUM:
+    case (int)M3_OP_RMS_NORM_E4M3:
+    case (int)M3_OP_VERIFY_DRAFT:
         return true;
     default:
         return false;
     }
+}
+
+bool m3c_kind_session_only(m3_op_kind kind)
+{
+    return kind == M3_OP_RMS_NORM_E4M3 || kind == M3_OP_VERIFY_DRAFT;
 }
 
 const char *m3c_kind_name(m3_op_kind kind)
@@ -610,6 +761,8 @@ const char *m3c_kind_name(m3_op_kind kind)
     case (int)M3_OP_ABS_MAX: return "ABS_MAX";
     case (int)M3_OP_CLAMP_UNIT: return "CLAMP_UNIT";
     case (int)M3_OP_ROW_SUM: return "ROW_SUM";
+    case (int)M3_OP_RMS_NORM_E4M3: return "RMS_NORM_E4M3";
+    case (int)M3_OP_VERIFY_DRAFT: return "VERIFY_DRAFT";
     default: return "UNSUPPORTED";
     }
 }
@@ -661,6 +814,12 @@ m3_status m3c_validate(const m3c_vcommand *command, m3_error *error)
         break;
     case (int)M3_OP_ROW_SUM:
         status = validate_row_sum(command, error);
+        break;
+    case (int)M3_OP_RMS_NORM_E4M3:
+        status = validate_norm_e4m3(command, error);
+        break;
+    case (int)M3_OP_VERIFY_DRAFT:
+        status = validate_verify(command, error);
         break;
     default:
         status = m3c_error_set(error, M3_STATUS_UNSUPPORTED,

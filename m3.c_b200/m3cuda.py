@@ -26,20 +26,23 @@ OK, INVALID_ARGUMENT, OUT_OF_RANGE, OVERFLOW, OUT_OF_MEMORY = 0, 1, 2, 3, 4
 IO, INVALID_FORMAT, UNSUPPORTED, CANCELLED, INTERNAL = 5, 6, 7, 8, 9
 # include/m3.h:45-50
 F32, F16, BF16, I32 = 0, 1, 2, 3
+E4M3 = 64  # CUDA extension
 # include/m3.h:52-73 and the CUDA extensions
 OPS = dict(COPY=0, CAST=1, ADD=2, MUL=3, EMBEDDING=4, MATMUL=5, LINEAR=6,
            RMS_NORM=7, LAYER_NORM=8, ROPE=9, ATTENTION=10, GATED_SILU=11,
            SOFTMAX=12, TOP_K=13, CATEGORICAL=14, CONV1D=15,
            CONV_TRANSPOSE1D=16, NEAREST_RESIZE1D=17, SNAKE1D=18, TANH=19,
-           ABS_MAX=64, CLAMP_UNIT=65, ROW_SUM=66)
+           ABS_MAX=64, CLAMP_UNIT=65, ROW_SUM=66, RMS_NORM_E4M3=67,
+           VERIFY_DRAFT=68)
 # include/m3.h:80-91
 PROVIDER_NEURAL_ENGINE, PROVIDER_METAL, PROVIDER_CPU, PROVIDER_CUDA = 0, 1, 2, 3
 INPUT, CONSTANT, TEMPORARY, OUTPUT = 0, 1, 2, 3
 VALUE_NONE = 0xFFFFFFFF
 MAX_RANK = 8
 
-NUMPY_OF = {F32: np.float32, F16: np.uint16, BF16: np.uint16, I32: np.int32}
-ITEMSIZE = {F32: 4, F16: 2, BF16: 2, I32: 4}
+NUMPY_OF = {F32: np.float32, F16: np.uint16, BF16: np.uint16, I32: np.int32,
+            E4M3: np.uint8}
+ITEMSIZE = {F32: 4, F16: 2, BF16: 2, I32: 4, E4M3: 1}
 
 
 class M3Error(ctypes.Structure):
@@ -573,7 +576,8 @@ class Graph:
         for i in range(2):
             desc.outputs[i] = VALUE_NONE
         for i, v in enumerate(inputs):
-            desc.inputs[i] = v
+            if v is not None:       # an optional input left out
+                desc.inputs[i] = v
         for i, v in enumerate(outputs):
             desc.outputs[i] = v
         if epsilon is not None:
@@ -589,7 +593,8 @@ class Graph:
         check(self.lib.m3_graph_add_node(self.handle, ctypes.byref(desc),
                                          ctypes.byref(err)), err)
 
-    def _shape_of(self, kind: int, inputs: list[int], k: int | None):
+    def _shape_of(self, kind: int, inputs: list[int], k: int | None,
+                  output_index: int = 0):
         """Python-side copy of the inferred shape, for read-buffer sizing."""
         first = self.values[inputs[0]][1]
         if kind in (OPS["ADD"], OPS["MUL"]):
@@ -602,6 +607,10 @@ class Graph:
             return first[:-1] + (1,)
         if kind == OPS["CATEGORICAL"]:
             return first[:-1]
+        if kind == OPS["RMS_NORM_E4M3"] and output_index == 1:
+            return first[:-1] + (1,)
+        if kind == OPS["VERIFY_DRAFT"]:
+            return first[:2] if output_index == 0 else first[:1]
         return first
 
     def inferred(self, kind: str | int, inputs: Iterable[int], role: int,
@@ -621,10 +630,12 @@ class Graph:
             dtype = self.values[inputs[0]][0]
         elif code == OPS["TOP_K"]:
             dtype = F32 if output_index == 0 else I32
-        elif code == OPS["CATEGORICAL"]:
+        elif code in (OPS["CATEGORICAL"], OPS["VERIFY_DRAFT"]):
             dtype = I32
-        self.values.append((dtype, self._shape_of(code, inputs,
-                                                  params.get("k")), role))
+        elif code == OPS["RMS_NORM_E4M3"]:
+            dtype = E4M3 if output_index == 0 else F32
+        self.values.append((dtype, self._shape_of(code, inputs, params.get("k"),
+                                                  output_index), role))
         return out.value
 
 

@@ -958,3 +958,172 @@ def test_step_captured_and_replayed(m3, gpu):
             graph.replay()
         for s in states:
             check_step(m3, s)
+
+
+# ------------------------------------------------------------- graph sessions
+
+def raw(t):
+    """A tensor as the session writes it: F32, or the 16-bit words."""
+    import torch
+
+    return t.cpu().numpy() if t.dtype in (torch.float32, torch.int32) else t.view(torch.int16).cpu().numpy()
+
+
+def norm_session(m3, x, w, group, r=None, keep_sum=False, **options):
+    import torch
+
+    dtype = {torch.float32: m3.F32, torch.float16: m3.F16, torch.bfloat16: m3.BF16}
+    shape = (2, x.shape[0] // 2, x.shape[1])
+    g = m3.Graph()
+    vx = g.value(m3.INPUT, dtype[x.dtype], shape)
+    vr = vh = None
+    h = vx
+    if r is not None:
+        vr = g.value(m3.INPUT, dtype[x.dtype], shape)
+        h = vh = g.inferred("ADD", [vx, vr], m3.OUTPUT if keep_sum else m3.TEMPORARY, dtype[x.dtype])
+        g.node("ADD", [vx, vr], [vh])
+    vw = g.value(m3.INPUT, dtype[w.dtype], (x.shape[1],))
+    codes = g.inferred("RMS_NORM_E4M3", [h, vw], m3.OUTPUT, m3.E4M3, epsilon=1e-6)
+    scales = g.value(m3.OUTPUT, m3.F32, shape[:2] + (x.shape[1] // group,))
+    g.node("RMS_NORM_E4M3", [h, vw], [codes, scales], epsilon=1e-6)
+    s = m3.Session(g, **options)
+    s.write(vx, raw(x))
+    s.write(vw, raw(w))
+    if vr is not None:
+        s.write(vr, raw(r))
+    return s, codes, scales, vh
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows, width, group", [(2, 64, 64), (64, 2048, 128), (10, 515, 515), (6, 4104, 24)])
+@pytest.mark.parametrize("residual", [None, "kept", "dropped"])
+def test_norm_in_a_session(m3, gpu, dtype, rows, width, group, residual):
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(width)
+    t = torch_dtype(dtype)
+    x = torch.randn(rows, width, generator=g, device="cuda").to(t)
+    r = torch.randn(rows, width, generator=g, device="cuda").to(t) if residual else None
+    w = torch.randn(width, generator=g, device="cuda").to(t)
+    codes, scales = run_norm(m3, x, w, group, r, None)
+    for options in (dict(), dict(fuse=False), dict(cuda_graphs=False)):
+        s, vc, vs, vh = norm_session(m3, x, w, group, r, residual == "kept", **options)
+        for _ in range(2):
+            s.run()
+        s.run_async()
+        s.run_async()
+        s.synchronize()
+        assert np.array_equal(s.read(vc).reshape(rows, width), codes.cpu().numpy())
+        assert np.array_equal(s.read(vs).reshape(rows, -1), scales.cpu().numpy())
+        if residual == "kept":
+            h = (x.float() + r.float()).to(t)
+            assert np.array_equal(s.read(vh).reshape(rows, width).view(raw(h).dtype), raw(h))
+        s.close()
+
+
+def test_norm_split_over_rows(m3, gpu):
+    """Two shards of one graph on this GPU give the whole graph's results."""
+    import torch
+
+    x = torch.randn(8, 2, 256, device="cuda").bfloat16()
+    w = torch.randn(256, device="cuda")
+    whole = run_norm(m3, x.view(16, 256), w, 64)
+    codes, scales = np.zeros((8, 2, 256), np.uint8), np.zeros((8, 2, 4), np.float32)
+    for rank in (0, 1):
+        g = m3.Graph()
+        vx, vw = g.value(m3.INPUT, m3.BF16, (8, 2, 256)), g.value(m3.INPUT, m3.F32, (256,))
+        vc = g.inferred("RMS_NORM_E4M3", [vx, vw], m3.OUTPUT, m3.E4M3, epsilon=1e-6)
+        vs = g.value(m3.OUTPUT, m3.F32, (8, 2, 4))
+        g.node("RMS_NORM_E4M3", [vx, vw], [vc, vs], epsilon=1e-6)
+        s = m3.Session(g, shard=m3.ShardOptions(rank, 2, 0))
+        hx = np.ascontiguousarray(raw(x))
+        s.shard_write(vx, hx.ctypes.data, hx.nbytes)
+        s.write(vw, raw(w))
+        s.run()
+        s.shard_read(vc, codes.ctypes.data, codes.nbytes)
+        s.shard_read(vs, scales.ctypes.data, scales.nbytes)
+    assert np.array_equal(codes.reshape(16, 256), whole[0].cpu().numpy())
+    assert np.array_equal(scales.reshape(16, 4), whole[1].cpu().numpy())
+
+
+@pytest.mark.parametrize("drawn", [True, False])
+@pytest.mark.parametrize("ragged", [True, False])
+def test_verify_behind_softmax_in_a_session(m3, gpu, drawn, ragged):
+    """SOFTMAX of the logits, then VERIFY_DRAFT, in one graph; a NaN logit fails the run before it."""
+    import torch
+
+    batch, drafts, vocabulary = 6, 3, 1000
+    rng = np.random.default_rng(3)
+    logits = rng.normal(size=(batch, drafts + 1, vocabulary)).astype(np.float32) * 2
+    tokens = rng.integers(0, vocabulary, (batch, drafts)).astype(np.int32)
+    tokens[2:] = logits[2:, :drafts].argmax(-1)
+    uniforms = rng.uniform(0, 0.05, (batch, drafts + 1)).astype(np.float32)
+    lengths = np.array([3, 0, 3, 1, 2, -1], np.int32)
+    g = m3.Graph()
+    vl = g.value(m3.INPUT, m3.F32, logits.shape)
+    p = g.inferred("SOFTMAX", [vl], m3.OUTPUT, m3.F32)
+    g.node("SOFTMAX", [vl], [p])
+    vt, vu = g.value(m3.INPUT, m3.I32, tokens.shape), g.value(m3.INPUT, m3.F32, uniforms.shape)
+    vq = g.value(m3.INPUT, m3.F32, (batch, drafts, vocabulary)) if drawn else None
+    vn = g.value(m3.INPUT, m3.I32, (batch,)) if ragged else None
+    ins = [p, vt, vu, vq, vn]
+    out = g.inferred("VERIFY_DRAFT", ins, m3.OUTPUT, m3.I32, 0)
+    accepted = g.inferred("VERIFY_DRAFT", ins, m3.OUTPUT, m3.I32, 1)
+    g.node("VERIFY_DRAFT", ins, [out, accepted])
+    s = m3.Session(g)
+    assert s.plan_report()[1] == "row[SOFTMAX]; row[VERIFY_DRAFT]"
+    q = np.full((batch, drafts, vocabulary), 1.0 / vocabulary, np.float32)
+    for value, data in ((vl, logits), (vt, tokens), (vu, uniforms), (vq, q), (vn, lengths)):
+        if value is not None:
+            s.write(value, data)
+    s.run()
+    target = s.read(p).astype(np.float64)
+    want = verify_host(target, q.astype(np.float64) if drawn else None, tokens, lengths if ragged else None,
+                       uniforms.astype(np.float64))
+    assert np.array_equal(s.read(out), want[0]) and np.array_equal(s.read(accepted), want[1])
+    assert want[1].max() > 0
+    # a failing run leaves the outputs as they were
+    bad = logits.copy()
+    bad[1, 1, 5] = np.nan
+    s.write(vl, bad)
+    s.write(vu, uniforms / 2)
+    status, message = s.run_status()
+    assert status == m3.OUT_OF_RANGE and "softmax" in message
+    assert np.array_equal(s.read(out), want[0]) and np.array_equal(s.read(accepted), want[1])
+    s.write(vl, logits)
+    s.run()
+    want = verify_host(target, q.astype(np.float64) if drawn else None, tokens, lengths if ragged else None,
+                       uniforms.astype(np.float64) / 2)
+    assert np.array_equal(s.read(out), want[0]) and np.array_equal(s.read(accepted), want[1])
+
+
+def test_empty_batches_in_a_session(m3, gpu):
+    """No rows, no sequences: the runs still count as started, and later ones work."""
+    g = m3.Graph()
+    x, w = g.value(m3.INPUT, m3.F32, (0, 64)), g.value(m3.INPUT, m3.F32, (64,))
+    codes = g.inferred("RMS_NORM_E4M3", [x, w], m3.OUTPUT, m3.E4M3, epsilon=1e-6)
+    scales = g.inferred("RMS_NORM_E4M3", [x, w], m3.OUTPUT, m3.F32, 1, epsilon=1e-6)
+    g.node("RMS_NORM_E4M3", [x, w], [codes, scales], epsilon=1e-6)
+    target, tokens = g.value(m3.INPUT, m3.F32, (0, 4, 100)), g.value(m3.INPUT, m3.I32, (0, 3))
+    uniforms = g.value(m3.INPUT, m3.F32, (0, 4))
+    out = g.inferred("VERIFY_DRAFT", [target, tokens, uniforms], m3.OUTPUT, m3.I32, 0)
+    accepted = g.inferred("VERIFY_DRAFT", [target, tokens, uniforms], m3.OUTPUT, m3.I32, 1)
+    g.node("VERIFY_DRAFT", [target, tokens, uniforms], [out, accepted])
+    s = m3.Session(g)
+    s.run()
+    s.run()
+    assert s.read(codes).shape == (0, 64) and s.read(accepted).shape == (0,)
+
+
+def test_plugin_refuses_session_operators(m3, gpu):
+    import ctypes
+
+    lib, err, context = m3.load(), m3.M3Error(), ctypes.c_void_p()
+    accessor = m3.STORAGE_DATA(lambda storage: storage)
+    options = m3.BackendOptions(0, accessor, False)
+    m3.check(lib.m3_cuda_backend_context_create(ctypes.byref(options), ctypes.byref(context), ctypes.byref(err)), err)
+    for kind in ("RMS_NORM_E4M3", "VERIFY_DRAFT"):
+        commands = (m3.Command * 1)()
+        commands[0].kind = m3.OPS[kind]
+        assert lib.m3_cuda_backend_execute(context, commands, 1, None, ctypes.byref(err)) == m3.UNSUPPORTED
+    lib.m3_cuda_backend_destroy_context(context)

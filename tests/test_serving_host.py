@@ -139,3 +139,139 @@ def test_cache_null(m3):
     assert lib.m3_cuda_cache_synchronize(None, None, err) == m3.INVALID_ARGUMENT
     assert lib.m3_cuda_cache_device_pointers(None, None, None, None, None, err) == m3.INVALID_ARGUMENT
     lib.m3_cuda_cache_free(None)
+
+
+# ------------------------------------------------------------ graph operators
+
+def norm_graph(m3, shape=(6, 4, 128), groups=1, dtype=None, residual=False, role=None):
+    g = m3.Graph()
+    dtype = m3.BF16 if dtype is None else dtype
+    x = g.value(m3.INPUT, dtype, shape)
+    if residual:
+        r = g.value(m3.INPUT, dtype, shape)
+        h = g.inferred("ADD", [x, r], m3.TEMPORARY if role is None else role, dtype)
+        g.node("ADD", [x, r], [h])
+    else:
+        h = x
+    w = g.value(m3.INPUT, m3.F32, shape[-1:])
+    codes = g.inferred("RMS_NORM_E4M3", [h, w], m3.OUTPUT, m3.E4M3, epsilon=1e-6)
+    scales = g.value(m3.OUTPUT, m3.F32, shape[:-1] + (groups,))
+    return g, (h, w), (codes, scales)
+
+
+def test_norm_node_plans(m3):
+    for residual, text in ((False, "row[RMS_NORM_E4M3]"), (True, "row[ADD+RMS_NORM_E4M3]")):
+        g, ins, outs = norm_graph(m3, residual=residual, groups=4)
+        g.node("RMS_NORM_E4M3", ins, outs, epsilon=1e-6)
+        info, report, described = m3.graph_plan(g)
+        assert described == text and report.launch_count == 1 and report.shadow_bytes == 0
+        if residual:
+            _, report, described = m3.graph_plan(g, fuse=False)
+            assert described == "ew[ADD] stores=1; row[RMS_NORM_E4M3]" and report.launch_count == 2
+    # one byte per code: 6 * 4 * 128 codes next to the inputs, the sum and the scales
+    assert info.allocated_bytes == 6 * 4 * 128 * (2 + 2 + 2 + 1) + 128 * 4 + 6 * 4 * 4 * 4
+
+
+def test_norm_node_inference(m3):
+    g, ins, _ = norm_graph(m3)
+    assert g.values[-2][:2] == (m3.E4M3, (6, 4, 128))
+    scales = g.inferred("RMS_NORM_E4M3", ins, m3.OUTPUT, m3.F32, 1, epsilon=1e-6)
+    assert g.values[scales][:2] == (m3.F32, (6, 4, 1))
+    refused(m3, lambda: g.inferred("RMS_NORM_E4M3", ins, m3.OUTPUT, m3.F32, 2), m3.OUT_OF_RANGE, "no requested")
+    refused(m3, lambda: g.inferred("RMS_NORM", ins, m3.OUTPUT, m3.F32, 1), m3.OUT_OF_RANGE, "no requested")
+
+
+@pytest.mark.parametrize("change, text", [
+    (dict(epsilon=0.0), "epsilon is invalid"),
+    (dict(groups=3), "groups dividing"),
+    (dict(groups=0), "groups dividing"),
+    (dict(scales=(24, 4)), "groups dividing"),
+    (dict(codes_dtype="F32"), "codes must be E4M3"),
+    (dict(scales_dtype="BF16"), "codes must be E4M3"),
+    (dict(weight=(64,)), "channel shape"),
+    (dict(dtype="I32"), "floating-point"),
+])
+def test_norm_node_refusals(m3, change, text):
+    g = m3.Graph()
+    x = g.value(m3.INPUT, getattr(m3, change.get("dtype", "F16")), (6, 4, 128))
+    w = g.value(m3.INPUT, m3.F32, change.get("weight", (128,)))
+    codes = g.value(m3.OUTPUT, getattr(m3, change.get("codes_dtype", "E4M3")), (6, 4, 128))
+    scales = g.value(m3.OUTPUT, getattr(m3, change.get("scales_dtype", "F32")),
+                     change.get("scales", (6, 4, change.get("groups", 1))))
+    g.node("RMS_NORM_E4M3", [x, w], [codes, scales], epsilon=change.get("epsilon", 1e-6))
+    refused(m3, lambda: m3.graph_plan(g), m3.INVALID_ARGUMENT, text)
+
+
+def test_no_other_operator_takes_e4m3(m3):
+    for kind, status in (("COPY", m3.UNSUPPORTED), ("CAST", m3.UNSUPPORTED), ("SOFTMAX", m3.INVALID_ARGUMENT),
+                         ("TANH", m3.INVALID_ARGUMENT), ("ABS_MAX", m3.INVALID_ARGUMENT),
+                         ("ROW_SUM", m3.INVALID_ARGUMENT), ("CLAMP_UNIT", m3.INVALID_ARGUMENT)):
+        g = m3.Graph()
+        x = g.value(m3.INPUT, m3.E4M3, (4, 8))
+        out = g.value(m3.OUTPUT, m3.E4M3 if kind == "COPY" else m3.F32, (4, 8))
+        g.node(kind, [x], [out])
+        with pytest.raises(m3.M3Failure) as failure:
+            m3.graph_plan(g)
+        assert failure.value.status == status, (kind, failure.value)
+    for dtype in (4, 63, 65, -1):
+        with pytest.raises(m3.M3Failure):
+            m3.Graph().value(m3.INPUT, dtype, (4,))
+
+
+def verify_graph(m3, batch=3, drafts=4, vocabulary=50, drawn=True, lengths=True, **change):
+    g = m3.Graph()
+    dtype = getattr(m3, change.get("dtype", "F32"))
+    ins = [g.value(m3.INPUT, dtype, change.get("target", (batch, drafts + 1, vocabulary))),
+           g.value(m3.INPUT, getattr(m3, change.get("tokens_dtype", "I32")), change.get("tokens", (batch, drafts))),
+           g.value(m3.INPUT, getattr(m3, change.get("uniforms_dtype", "F32")),
+                   change.get("uniforms", (batch, drafts + 1))),
+           g.value(m3.INPUT, getattr(m3, change.get("draft_dtype", change.get("dtype", "F32"))),
+                   change.get("draft", (batch, drafts, vocabulary))) if drawn else None,
+           g.value(m3.INPUT, getattr(m3, change.get("lengths_dtype", "I32")), change.get("lengths_shape", (batch,)))
+           if lengths else None]
+    outs = [g.value(m3.OUTPUT, m3.I32, change.get("out", (batch, drafts + 1))),
+            g.value(m3.OUTPUT, m3.I32, change.get("accepted", (batch,)))]
+    g.node("VERIFY_DRAFT", ins, outs)
+    return g, ins, outs
+
+
+def test_verify_node_plans(m3):
+    for drawn in (False, True):
+        for lengths in (False, True):
+            g, ins, _ = verify_graph(m3, drawn=drawn, lengths=lengths)
+            _, report, described = m3.graph_plan(g)
+            assert described == "row[VERIFY_DRAFT]" and report.shadow_bytes == 0
+    tokens = g.inferred("VERIFY_DRAFT", ins, m3.OUTPUT, m3.I32, 0)
+    accepted = g.inferred("VERIFY_DRAFT", ins, m3.OUTPUT, m3.I32, 1)
+    assert g.values[tokens][:2] == (m3.I32, (3, 5)) and g.values[accepted][:2] == (m3.I32, (3,))
+
+
+@pytest.mark.parametrize("change, text", [
+    (dict(dtype="I32"), "dtype"), (dict(tokens_dtype="F32"), "dtype"), (dict(uniforms_dtype="BF16"), "dtype"),
+    (dict(draft_dtype="F16"), "dtype"), (dict(lengths_dtype="F32"), "dtype"),
+    (dict(target=(3, 250)), "shape"), (dict(target=(3, 5, 0)), "shape"), (dict(tokens=(3, 5)), "shape"),
+    (dict(tokens=(12,)), "shape"), (dict(uniforms=(3, 4)), "shape"), (dict(draft=(3, 5, 50)), "shape"),
+    (dict(draft=(3, 4, 51)), "shape"), (dict(lengths_shape=(3, 1)), "shape"), (dict(out=(3, 4)), "shape"),
+    (dict(accepted=(3, 1)), "shape"),
+])
+def test_verify_node_refusals(m3, change, text):
+    g, _, _ = verify_graph(m3, **change)
+    refused(m3, lambda: m3.graph_plan(g), m3.INVALID_ARGUMENT, f"verification {text} is invalid")
+
+
+def test_serving_nodes_are_the_sessions_own(m3):
+    lib = m3.load()
+    for kind in ("RMS_NORM_E4M3", "VERIFY_DRAFT"):
+        assert not lib.m3_cuda_backend_supports_kind(m3.OPS[kind])
+    assert lib.m3_cuda_backend_supports_kind(m3.OPS["RMS_NORM"])
+
+
+def test_serving_nodes_split(m3):
+    g, ins, outs = norm_graph(m3, shape=(8, 4, 128), groups=4)
+    g.node("RMS_NORM_E4M3", ins, outs, epsilon=1e-6)
+    for rank in (0, 1):
+        slab, axis = m3.shard_plan(g, rank, 2, -1, outs[1])
+        assert axis == 0 and slab.split and slab.begin == 4 * rank and slab.extent == 4
+    refused(m3, lambda: m3.shard_plan(g, 0, 2, 2, outs[0]), m3.UNSUPPORTED, "axis 2")
+    g, _, outs = verify_graph(m3)
+    refused(m3, lambda: m3.shard_plan(g, 0, 2, 0, outs[0]), m3.UNSUPPORTED, "VERIFY_DRAFT (node 0) cannot be sharded")
