@@ -4,6 +4,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "m3c_device.cuh"
@@ -34,10 +35,13 @@ __device__ __forceinline__ uint32_t warp_max(uint32_t v)
 // SMs of the current device.
 int sm_count()
 {
+    static std::atomic<int> known[64];
     int device = 0;
-    int sms = 148;
-    if (cudaGetDevice(&device) == cudaSuccess) {
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return 148;
+    int sms = known[device].load(std::memory_order_relaxed);
+    if (sms == 0) {
+        if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms <= 0) sms = 148;
+        known[device].store(sms, std::memory_order_relaxed);
     }
     return sms;
 }
@@ -262,11 +266,33 @@ __device__ __forceinline__ void multiply(float (&a)[N], float b)
     multiply(a, all);
 }
 
+// The divisor of a group whose largest |z| is `most`.  A code is that of y / s =
+// (z inverse) / s, and as s is the group's largest |y| / 448, that of z over the
+// largest |z| / 448: the inverse root drops out, and with it two roundings.
+// Where a scale is at its lower bound, or not finite, the quotient is taken of y
+// itself (`normed`).
+struct norm_divisor {
+    e4m3_divisor by;
+    float scale;
+    bool normed;
+};
+
+__device__ __forceinline__ norm_divisor divide_norm_by(float most, float inverse)
+{
+    norm_divisor d;
+    const float of_z = e4m3_scale(magnitude_bits(most));
+    d.scale = __fmul_rn(of_z, inverse);
+    d.normed = !(of_z > E4M3_SMALLEST_SCALE && d.scale > E4M3_SMALLEST_SCALE);  // a NaN too
+    if (d.normed) d.scale = e4m3_scale(magnitude_bits(__fmul_rn(most, inverse)));
+    d.by = e4m3_divide_by(d.normed ? d.scale : of_z);
+    return d;
+}
+
 // The most threads of a row: the register kernel's widest rows are VEC * K times
 // as many elements.
 constexpr int norm_block(int vec, int k)
 {
-    return vec == 1 ? 512 : k == 1 ? 1024 : k == 2 ? 512 : 256;
+    return vec == 1 || k == 1 ? 1024 : k == 2 ? 512 : 256;
 }
 
 template <int DT, int MODE, int VEC, int K>
@@ -390,9 +416,9 @@ __global__ void __launch_bounds__(norm_block(VEC, K))
     }
     if (!live) return;
     const float inverse = __frsqrt_rn(__fadd_rn(__fdiv_rn(squares[0], static_cast<float>(width)), p.epsilon));
-    e4m3_divisor d = {};
+    norm_divisor d;
     if constexpr (MODE == GROUP_ROW) {
-        d = e4m3_divide_by(e4m3_scale(magnitude_bits(__fmul_rn(as_float(largest), inverse))));
+        d = divide_norm_by(as_float(largest), inverse);
         if (tid == 0) p.code_scales[row] = d.scale;
     }
     uint8_t *codes = static_cast<uint8_t *>(p.codes) + row * width;
@@ -403,11 +429,11 @@ __global__ void __launch_bounds__(norm_block(VEC, K))
         if constexpr (MODE != GROUP_ROW) {
             const uint32_t g = group_of(at);
             if constexpr (MODE == GROUP_WORDS) most[k] = as_float(words[place + g]);
-            d = e4m3_divide_by(e4m3_scale(magnitude_bits(__fmul_rn(most[k], inverse))));
+            d = divide_norm_by(most[k], inverse);
             if (at == g * group) p.code_scales[row * groups + g] = d.scale;
         }
-        multiply(z[k], inverse);
-        e4m3_store<VEC>(codes + at, z[k], d);
+        if (d.normed) multiply(z[k], inverse);
+        e4m3_store<VEC>(codes + at, z[k], d.by);
     }
 }
 
@@ -450,12 +476,12 @@ __global__ void __launch_bounds__(QUANT_THREADS)
         for (int w = 0; w < QUANT_WARPS; ++w) squares = __fadd_rn(squares, part[w]);
         const float inverse =
             __frsqrt_rn(__fadd_rn(__fdiv_rn(squares, static_cast<float>(p.width)), p.epsilon));
-        auto normed = [&](uint64_t j) {
+        auto weighted = [&](uint64_t j) {
             // the stored sum is h (and may be the input's own storage by now)
             const float h = kept                   ? held[j]
                             : p.sum_out != nullptr ? load_element(p.sum_out, p.dtype, s0 + j)
                                                    : read(j);
-            return __fmul_rn(__fmul_rn(h, load_element(p.scale, p.scale_dtype, j)), inverse);
+            return __fmul_rn(h, load_element(p.scale, p.scale_dtype, j));
         };
         uint8_t *codes = static_cast<uint8_t *>(p.codes) + row * p.width;
         // many groups: one warp each; few: the whole CTA one after another
@@ -466,7 +492,7 @@ __global__ void __launch_bounds__(QUANT_THREADS)
             const uint64_t g0 = g * p.group;
             uint32_t largest = 0u;
             for (uint64_t j = from; j < p.group; j += step) {
-                const uint32_t m = magnitude_bits(normed(g0 + j));
+                const uint32_t m = magnitude_bits(weighted(g0 + j));
                 largest = m > largest ? m : largest;
             }
             largest = warp_max(largest);
@@ -475,9 +501,12 @@ __global__ void __launch_bounds__(QUANT_THREADS)
                 __syncthreads();
                 for (int w = 0; w < QUANT_WARPS; ++w) largest = top[w] > largest ? top[w] : largest;
             }
-            const e4m3_divisor d = e4m3_divide_by(e4m3_scale(largest));
+            const norm_divisor d = divide_norm_by(as_float(largest), inverse);
             if (from == 0) p.code_scales[row * groups + g] = d.scale;
-            for (uint64_t j = from; j < p.group; j += step) codes[g0 + j] = e4m3_code(normed(g0 + j), d);
+            for (uint64_t j = from; j < p.group; j += step) {
+                const float z = weighted(g0 + j);
+                codes[g0 + j] = e4m3_code(d.normed ? __fmul_rn(z, inverse) : z, d.by);
+            }
             if (!alone) __syncthreads();
         }
         __syncthreads();
@@ -506,13 +535,21 @@ int norm_launch(const m3c_norm_e4m3_params &p, cudaStream_t stream)
 template <int DT, int MODE>
 int norm_depth(const m3c_norm_e4m3_params &p, bool vectors, cudaStream_t stream)
 {
-    if (!vectors) return norm_launch<DT, MODE, 1, 16>(p, stream);
-    // pieces per thread: two keep a row of 4096 elements in 256 threads; wider
-    // rows take more, unless there are too few rows to fill the SMs with
-    // their fewer threads
+        // single elements: 333 rows of 2051 F32 take 5.7 us with four per thread, 6.4
+    // with eight, which are for the widths past 1024 threads
+    if (!vectors && p.width <= 4096u) return norm_launch<DT, MODE, 1, 4>(p, stream);
+    if (!vectors) return norm_launch<DT, MODE, 1, 8>(p, stream);
+    // pieces per thread.  What a thread does once per row (the root, the
+    // divisor) weighs on two pieces: many rows of one group take four (16384 x
+    // 4096 bf16 without residual: 52 us against 57).  With a divisor per
+    // piece, or too few rows to fill the SMs with a row's fewer threads, two
+    // are faster (the same rows in groups of 128: 86 us against 90), as with
+    // F32's wider pieces (8192 x 4096 with residual: 70 us against 72).  Rows
+    // past 8192 elements need eight
     const uint64_t pieces = p.width / 8u;
+    const bool many = p.rows >= 2048u && MODE == GROUP_ROW && DT != M3C_F32;
     if (pieces <= 32u) return norm_launch<DT, MODE, 8, 1>(p, stream);
-    if (pieces <= 512u || (pieces <= 1024u && p.rows < 2048u)) return norm_launch<DT, MODE, 8, 2>(p, stream);
+    if (pieces <= 64u || (pieces <= 1024u && !many)) return norm_launch<DT, MODE, 8, 2>(p, stream);
     if (pieces <= 1024u) return norm_launch<DT, MODE, 8, 4>(p, stream);
     return norm_launch<DT, MODE, 8, 8>(p, stream);
 }
@@ -591,7 +628,7 @@ struct cache_shape {
 };
 
 constexpr int CACHE_THREADS = 512;    // at most; 256 where the shape allows
-constexpr uint32_t CACHE_STEPS = 8;   // at most
+constexpr uint32_t CACHE_STEPS = 16;  // at most
 constexpr uint32_t CACHE_SLOTS = 128 * CACHE_STEPS;  // 256 threads, one head of eight elements
 
 // A thread's place in its block's rows.
@@ -781,17 +818,19 @@ int launch_cache_vectors(const m3c_cache_params &p, cudaStream_t stream)
     const uint32_t block = (shape.rows * threads + 31u) / 32u * 32u;
     const uint32_t chunks = (all - 1u) / shape.vectors + 1u;
     const uint64_t groups = static_cast<uint64_t>((p.row_count - 1u) / shape.rows + 1u) * chunks;
-    const uint64_t waves = groups / (4u * static_cast<uint64_t>(sm_count()));  // of four CTAs per SM
+    const uint64_t resident = 4u * static_cast<uint64_t>(sm_count());  // CTAs at a time
     if constexpr (WRITE) {
-        // as many steps as leave every SM its CTAs
-        shape.steps = waves < 1u ? 1u : waves > CACHE_STEPS ? CACHE_STEPS : static_cast<uint32_t>(waves);
+        // whole waves of CTAs, each with as many steps as it may have
+        const uint64_t waves = (groups - 1u) / resident + 1u;
+        const uint64_t rounds = (waves - 1u) / CACHE_STEPS + 1u;
+        shape.steps = static_cast<uint32_t>((waves - 1u) / rounds + 1u);
         const dim3 grid((p.row_count - 1u) / (shape.rows * shape.steps) + 1u, chunks);
         cache_write_kernel<DT, P><<<grid, block, 0, stream>>>(p, shape);
     } else {
         // a small batch takes one: the unrolled code's own fetch costs more
         // than it hides
         constexpr int MANY = P == 1 ? 4 : 2;
-        shape.steps = waves < MANY ? 1u : MANY;
+        shape.steps = groups < MANY * resident ? 1u : MANY;
         const dim3 grid((p.row_count - 1u) / (shape.rows * shape.steps) + 1u, chunks);
         if (shape.steps == 1u) {
             cache_read_kernel<DT, P, 1><<<grid, block, 0, stream>>>(p, shape);
