@@ -940,7 +940,8 @@ m3_status m3_cuda_abs_max_static(int device, void *stream, m3_dtype dtype,
  *   y = h * scale / sqrt(mean(h^2) + epsilon)     (F32; the mean over the row)
  * and each `group` consecutive elements of a row of y quantised together.
  * The row sums run in F32 in a fixed order of their own (not the reference's
- * left-to-right order of M3_OP_RMS_NORM), so results repeat bit for bit.
+ * left-to-right order of M3_OP_RMS_NORM), so results repeat bit for bit; a row
+ * whose squares pass the F32 range has y = 0, as its infinite mean says.
  * `sum` (may be NULL) receives h.  It may be the very tensor `input` or
  * `residual` (same address and row stride); no other output may overlap an
  * input or another output (M3_STATUS_INVALID_ARGUMENT; the byte spans are
@@ -1027,15 +1028,17 @@ typedef struct {
 /* Quantise the rows' keys and values into their slots; each vector of head_dim
  * elements is one group.  No two rows of a call may name one slot, nor may
  * calls that overlap in time name a slot that one of them writes: its vectors
- * are then unspecified (all other slots hold what they should). */
+ * are then unspecified (all other slots hold what they should).  The rows'
+ * own vectors may overlap (they are only read). */
 m3_status m3_cuda_cache_write(m3_cuda_cache *cache, void *stream,
                               const m3_cuda_cache_batch *batch,
                               const m3_cuda_cache_rows *keys,
                               const m3_cuda_cache_rows *values,
                               m3_error *error);
 /* Read the rows' slots back: code * scale, in F32, rounded to the rows' dtype.
- * Several rows may name one slot (a shared prefix).  The vectors of `keys` and
- * `values` must not overlap each other (they may interleave). */
+ * Several rows may name one slot (a shared prefix).  No two vectors of `keys`
+ * and `values` may overlap (they may interleave): what overlaps is then
+ * unspecified. */
 m3_status m3_cuda_cache_read(m3_cuda_cache *cache, void *stream,
                              const m3_cuda_cache_batch *batch,
                              const m3_cuda_cache_rows *keys,
@@ -1044,7 +1047,9 @@ m3_status m3_cuda_cache_read(m3_cuda_cache *cache, void *stream,
 
 /* Wait for `stream`, then report (and forget) the first skipped row since the
  * last report: M3_STATUS_OUT_OF_RANGE, with the row and the reason in the
- * message. */
+ * message.  Rows skipped later, by work on other streams, are kept for the
+ * next report.  One synchronise of a cache at a time; writes and reads may be
+ * enqueued by several threads. */
 m3_status m3_cuda_cache_synchronize(m3_cuda_cache *cache, void *stream,
                                     m3_error *error);
 

@@ -268,6 +268,9 @@ typedef struct {
 
 int m3c_launch_cache_write(const m3c_cache_params *params, void *stream);
 int m3c_launch_cache_read(const m3c_cache_params *params, void *stream);
+/* *report = *first_skipped, which is cleared (all ones), in one exchange. */
+int m3c_launch_cache_report(unsigned long long *first_skipped,
+                            unsigned long long *report, void *stream);
 
 /* Verification of drafted tokens (m3_cuda_verify_draft). */
 typedef struct {

@@ -59,8 +59,11 @@ unsigned capped_grid(uint64_t wanted, unsigned per_sm)
 //   per group of y: scale, codes (m3c_e4m3.cuh).
 //
 // Bytes bound it: x and r in, h and the codes out, 7 bytes per element of a
-// 16-bit residual stream against some 14 instructions.  Both kernels below
-// read a row once and keep h on the SM until its codes are out.
+// 16-bit residual stream.  16384 x 4096 bf16 with residual: 74.4 us, 6.3 TB/s,
+// 0.96 of the measured copy rate; in groups of 128, which make a divisor per
+// eight elements, 85.8 us (0.84).  Without a residual, three bytes an element,
+// the instructions (some twelve an element) weigh more: 52 us (0.59).  Both
+// kernels below read a row once and keep h on the SM until its codes are out.
 
 // The register kernel: `threads` threads (whole warps) own a row, each K pieces
 // of VEC consecutive elements in registers, piece k of thread i being number
@@ -288,11 +291,10 @@ __device__ __forceinline__ norm_divisor divide_norm_by(float most, float inverse
     return d;
 }
 
-// The most threads of a row: the register kernel's widest rows are VEC * K times
-// as many elements.
+// The most threads of a CTA of the register kernel, as norm_depth chooses K.
 constexpr int norm_block(int vec, int k)
 {
-    return vec == 1 || k == 1 ? 1024 : k == 2 ? 512 : 256;
+    return vec == 1 ? 1024 : k == 1 ? NORM_THREADS : k == 2 ? 512 : 256;
 }
 
 template <int DT, int MODE, int VEC, int K>
@@ -535,8 +537,8 @@ int norm_launch(const m3c_norm_e4m3_params &p, cudaStream_t stream)
 template <int DT, int MODE>
 int norm_depth(const m3c_norm_e4m3_params &p, bool vectors, cudaStream_t stream)
 {
-        // single elements: 333 rows of 2051 F32 take 5.7 us with four per thread, 6.4
-    // with eight, which are for the widths past 1024 threads
+    // single elements: 333 rows of 2051 F32 take 5.7 us with four per thread and
+    // 6.4 with eight, which are for the widths that four leave past 1024 threads
     if (!vectors && p.width <= 4096u) return norm_launch<DT, MODE, 1, 4>(p, stream);
     if (!vectors) return norm_launch<DT, MODE, 1, 8>(p, stream);
     // pieces per thread.  What a thread does once per row (the root, the
@@ -591,8 +593,8 @@ __device__ __forceinline__ int64_t slot_in_sequence(const m3c_cache_params &p, u
 }
 
 // The slots of `count` consecutive rows, by one warp: the sequence of the first
-// by a 32-way search, the others' from there on (the sequences of a CTA's few
-// rows are the same or next to one another).
+// by a 32-way search (a step for 32 sequences, two for 1024), the others' from
+// there on.
 __device__ __forceinline__ void find_slots(const m3c_cache_params &p, uint32_t first, uint32_t count, int64_t *slots)
 {
     const uint32_t lane = threadIdx.x % 32u;
@@ -607,8 +609,20 @@ __device__ __forceinline__ void find_slots(const m3c_cache_params &p, uint32_t f
         high = min(low + step, high);
     }
     for (uint32_t r = lane; r < count; r += 32u) {
+        const int64_t row = static_cast<int64_t>(first) + r;
         uint32_t s = low;
-        while (s + 1u < p.sequences && p.offsets[s + 1u] <= static_cast<int64_t>(first + r)) ++s;
+        if (s + 1u < p.sequences && p.offsets[s + 1u] <= row) {
+            uint32_t end = p.sequences;
+            ++s;
+            while (end - s > 1u) {
+                const uint32_t middle = s + (end - s) / 2u;
+                if (p.offsets[middle] <= row) {
+                    s = middle;
+                } else {
+                    end = middle;
+                }
+            }
+        }
         slots[r] = slot_in_sequence(p, first + r, s);
     }
 }
@@ -618,8 +632,13 @@ __device__ __forceinline__ void find_slots(const m3c_cache_params &p, uint32_t f
 // eight elements each, piece j of lane l being number j * lanes + l.  A thread
 // keeps its place (keys or values, head, lane) for several rows; blockIdx.y
 // takes over where a row's vectors do not fit a block.  The slots of a CTA's
-// rows are found once, in shared memory.  Bytes bound both directions: three
-// per element of 16-bit rows.
+// rows are found once, in shared memory.
+//
+// Bytes bound both directions: three per element of 16-bit rows.  262144 rows
+// of 8 heads of 128 in bf16 are read in 250 us (6.5 TB/s, 0.98 of the measured
+// copy rate), 65536 written in 74.5 us (5.5 TB/s, 0.83), 16384 in 21.1 us (0.73).
+// Writing has some eleven instructions an element (the maximum over the vector,
+// a correctly rounded quotient) and the dependent loads that find a slot.
 struct cache_shape {
     uint32_t lane_shift;
     uint32_t vectors;       // of a row, in a block
@@ -658,7 +677,8 @@ struct cache_place {
 };
 
 // Writing: the CTA walks over its rows, the next rows' loads on their way while
-// one row's codes are made; the slots are found behind the first loads.
+// one row's codes are made; the slots are found behind the first loads.  (One
+// row a CTA, unrolled as reading is: 87 us for the 65536 rows above.)
 template <int DT, int P>
 __global__ void __launch_bounds__(CACHE_THREADS, 2)
     cache_write_kernel(const __grid_constant__ m3c_cache_params p, const __grid_constant__ cache_shape shape)
@@ -715,7 +735,10 @@ __global__ void __launch_bounds__(CACHE_THREADS, 2)
     }
 }
 
-// Reading: the slots first, then STEPS rows of a thread at once.
+// Reading: the slots first, then STEPS rows of a thread at once.  (Walking as
+// writing does: 254 us for the 262144 rows above, 19.9 against 19.0 for 16384.)
+// F32 rows are stored 32 bytes a lane: two stores of 16 filled their sectors in
+// halves, 278 us against 207 for 131072 rows.
 template <int DT, int P, int STEPS>
 __global__ void __launch_bounds__(CACHE_THREADS)
     cache_read_kernel(const __grid_constant__ m3c_cache_params p, const __grid_constant__ cache_shape shape)
@@ -847,7 +870,7 @@ template <int DT, bool WRITE>
 int launch_cache_pieces(const m3c_cache_params &p, cudaStream_t stream)
 {
     // four pieces of F32, or of rows held while the next are read, leave too few
-    // threads on an SM
+    // threads on an SM (65536 rows written: 82 us with four, 76 with two)
     constexpr int MOST = WRITE || DT == M3C_F32 ? 3 : 4;
     const uint32_t pieces = p.head_dim / 8u;
     int best = 1;
@@ -855,7 +878,7 @@ int launch_cache_pieces(const m3c_cache_params &p, cudaStream_t stream)
     for (int k = 1; k <= MOST; ++k) {
         uint32_t lanes = 1u;
         while (lanes * k < pieces) lanes <<= 1;
-        if (lanes * k - pieces <= idle) {
+        if (lanes <= 32u && lanes * k - pieces <= idle) {
             idle = lanes * k - pieces;
             best = k;
         }
@@ -868,12 +891,19 @@ int launch_cache_pieces(const m3c_cache_params &p, cudaStream_t stream)
     }
 }
 
+// The first skipped row, and none from here on.
+__global__ void cache_report_kernel(unsigned long long *first_skipped, unsigned long long *report)
+{
+    *report = atomicExch(first_skipped, ~0ull);
+}
+
 template <bool WRITE>
 int launch_cache(const m3c_cache_params &p, cudaStream_t stream)
 {
     const uint64_t vectors = static_cast<uint64_t>(p.row_count) * 2u * p.heads;
-    // a vector's lanes are at most a warp; the grid's y counts heads
-    bool fits = p.dtype[0] == p.dtype[1] && p.head_dim % 8u == 0u && p.head_dim <= 256u && p.heads <= 16384u;
+    // a vector's lanes are at most a warp of three pieces each; the grid's y
+    // counts heads
+    bool fits = p.dtype[0] == p.dtype[1] && p.head_dim % 8u == 0u && p.head_dim <= 768u && p.heads <= 16384u;
     for (int k = 0; k < 2; ++k) {
         fits = fits && aligned_to(p.rows[k], p.dtype[0] == M3C_F32 ? 32 : 16) && p.token_stride[k] % 8u == 0u &&
                p.head_stride[k] % 8u == 0u;
@@ -928,4 +958,10 @@ extern "C" int m3c_launch_cache_write(const m3c_cache_params *params, void *stre
 extern "C" int m3c_launch_cache_read(const m3c_cache_params *params, void *stream)
 {
     return m3c::launch_cache<false>(*params, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int m3c_launch_cache_report(unsigned long long *first_skipped, unsigned long long *report, void *stream)
+{
+    m3c::cache_report_kernel<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(first_skipped, report);
+    return static_cast<int>(cudaGetLastError());
 }

@@ -15,7 +15,8 @@ struct m3_cuda_cache {
     unsigned char *arena;
     uint8_t *codes[2];
     float *scales[2];
-    unsigned long long *first_skipped;   /* device */
+    unsigned long long *first_skipped;   /* device; the word behind it holds
+                                            a synchronise's copy */
     unsigned long long *seen;            /* pinned */
 };
 
@@ -226,7 +227,7 @@ m3_status m3_cuda_rms_norm_e4m3(int device, void *stream,
                     status = check_apart(&s[SUM], &s[SCALE], error);
                 }
             } else if (out != SUM || s[k].begin != s[SUM].begin ||
-                       s[k].stride != s[SUM].stride) {
+                       (s[k].stride != s[SUM].stride && args->rows > 1U)) {
                 status = check_apart(&s[out], &s[k], error);
             }
         }
@@ -567,19 +568,17 @@ m3_status m3_cuda_cache_synchronize(m3_cuda_cache *cache, void *stream,
     if (status != M3_STATUS_OK) {
         return status;
     }
-    code = cudaMemcpyAsync(cache->seen, cache->first_skipped, sizeof(seen),
-                           cudaMemcpyDeviceToHost, s);
+    code = (cudaError_t)m3c_launch_cache_report(cache->first_skipped,
+                                                cache->first_skipped + 1, s);
+    if (code == cudaSuccess) {
+        code = cudaMemcpyAsync(cache->seen, cache->first_skipped + 1,
+                               sizeof(seen), cudaMemcpyDeviceToHost, s);
+    }
     if (code == cudaSuccess) {
         code = cudaStreamSynchronize(s);
     }
     if (code == cudaSuccess) {
         seen = *cache->seen;
-        if (seen != CACHE_CLEAN) {
-            code = cudaMemsetAsync(cache->first_skipped, 0xff, sizeof(seen), s);
-            if (code == cudaSuccess) {
-                code = cudaStreamSynchronize(s);
-            }
-        }
     }
     if (code != cudaSuccess) {
         status = cuda_failure(error, code, "cache synchronise failed");

@@ -343,7 +343,8 @@ def laid_out(t, layout):
 SHAPES = [
     (1, 1, 1, 1, 5), (2, 3, 8, 3, 40), (7, 5, 80, 48, 90), (3, 8, 128, 16, 70), (33, 2, 64, 16, 9), (70, 1, 128, 64, 4),
     (1, 4, 256, 16, 100), (2, 2, 257, 7, 20), (2, 1, 320, 16, 33), (5, 3, 60, 1, 12), (3, 16, 192, 100, 30),
-    (1, 8, 128, 16, 1), (1, 1, 8, 16, 1000), (2, 3, 1032, 4, 9), (300, 2, 16, 8, 3),
+    (1, 8, 128, 16, 1), (1, 1, 8, 16, 1000), (2, 3, 1032, 4, 9), (300, 2, 16, 8, 3), (3, 2, 576, 16, 30),
+    (2, 1, 768, 16, 20), (2, 1, 776, 16, 20), (1500, 1, 8, 16, 2), (2, 20, 256, 32, 40),
 ]
 
 
@@ -523,6 +524,49 @@ def test_cache_rows_outside_the_sequences(m3, gpu):
         c.cache.synchronize()
     except m3.M3Failure as failure:
         assert failure.status == m3.OUT_OF_RANGE
+
+
+def test_cache_large_batches(m3, gpu):
+    """Enough rows that a CTA walks over many, the last of them few; mostly empty sequences."""
+    import torch
+
+    for heads, dim, page, tokens in ((8, 128, 64, 20011), (1, 8, 16, 100003), (5, 80, 48, 9001)):
+        sequences = 1000
+        rng = np.random.default_rng(dim)
+        c = m3.Cache(tokens // page + sequences + 1, page, heads, dim)
+        cuts = np.sort(rng.integers(0, tokens, sequences - 1))
+        cuts[100:400] = cuts[100]
+        cuts = np.sort(cuts)
+        offsets = np.concatenate([[0], cuts, [tokens]])
+        need = -(-np.diff(offsets) // page)
+        order = rng.permutation(tokens // page + sequences + 1)
+        table = np.full((sequences, int(need.max())), -1)
+        slots = np.empty(tokens, np.int64)
+        for s, at in enumerate(np.cumsum(need) - need):
+            table[s, :need[s]] = order[at:at + need[s]]
+            p = np.arange(offsets[s + 1] - offsets[s])
+            slots[offsets[s]:offsets[s + 1]] = table[s][p // page] * page + p % page
+        held = [torch.from_numpy(a.astype(np.int32)).cuda() for a in (table, offsets)]
+        batch = m3.CacheBatch(page_table=held[0].data_ptr(), page_table_stride=table.shape[1],
+                              offsets=held[1].data_ptr(), starts=None, sequences=sequences, rows=tokens)
+        rows = torch.randn(2, tokens, heads, dim, device="cuda").bfloat16()
+        out = torch.zeros_like(rows)
+        c.write(batch, cache_rows(m3, rows[0]), cache_rows(m3, rows[1]))
+        c.read(batch, cache_rows(m3, out[0]), cache_rows(m3, out[1]))
+        c.synchronize()
+        for k in range(2):
+            v = rows[k].float()
+            scale = (v.abs().amax(-1) / 448).clamp_min(TINY)
+            # one place in a thousand is checked for its bits, all for their range
+            places = rng.integers(0, tokens, 64)
+            want_scale, value = quantised(host(rows[k][torch.from_numpy(places)]))
+            got = device_view(c.pointers()[2 * k], (c.shape[0] * page, heads, dim), "|u1")
+            at = torch.from_numpy(slots[places]).cuda()
+            assert np.array_equal(e4m3_table()[got[at].cpu().numpy()], value)
+            want = torch.from_numpy(value.astype(np.float32) * want_scale[..., None]).bfloat16()
+            assert torch.equal(out[k][torch.from_numpy(places)].cpu(), want)
+            # half a step of the largest binade, 16, and the value's own rounding to bf16
+            assert bool(((out[k].float() - v).abs() <= scale[..., None] * (16 + 448 * 2 ** -8 + 1e-3)).all())
 
 
 def test_cache_shared_prefix_and_one_slot_twice(m3, gpu):
