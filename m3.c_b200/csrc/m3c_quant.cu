@@ -204,17 +204,19 @@ __device__ __forceinline__ void add_piece(Piece<DT, VEC> &a, const Piece<DT, VEC
     }
 }
 
-// VEC weights; the same for every row, they stay in the caches.  16-bit ones are
-// read with the row, F32 ones, which take twice the registers, when used.
+// VEC weights; the same for every row, they stay in the caches.  They are read
+// with the row, but for eight F32 ones, which take twice the registers and are
+// read when used.
 template <int VEC>
 struct Weights {
     Piece<M3C_F16, VEC> early;
 
     __device__ __forceinline__ void load(const void *scale, int dtype, uint32_t element)
     {
-        if (dtype == M3C_F32) return;
         const uint16_t *from = static_cast<const uint16_t *>(scale) + element;
-        if constexpr (VEC == 8) {
+        if (dtype == M3C_F32) {
+            if constexpr (VEC == 1) early.w[0] = __ldg(static_cast<const uint32_t *>(scale) + element);
+        } else if constexpr (VEC == 8) {
             const uint4 q = __ldg(reinterpret_cast<const uint4 *>(from));
             early.w[0] = q.x, early.w[1] = q.y, early.w[2] = q.z, early.w[3] = q.w;
         } else {
@@ -232,7 +234,7 @@ struct Weights {
                 x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
                 x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
             } else {
-                x[0] = __ldg(from);
+                x[0] = as_float(early.w[0]);
             }
             return;
         }
@@ -537,7 +539,7 @@ int norm_launch(const m3c_norm_e4m3_params &p, cudaStream_t stream)
 template <int DT, int MODE>
 int norm_depth(const m3c_norm_e4m3_params &p, bool vectors, cudaStream_t stream)
 {
-    // single elements: 333 rows of 2051 F32 take 5.7 us with four per thread and
+    // single elements: 333 rows of 2051 F32 take 5.4 us with four per thread and
     // 6.4 with eight, which are for the widths that four leave past 1024 threads
     if (!vectors && p.width <= 4096u) return norm_launch<DT, MODE, 1, 4>(p, stream);
     if (!vectors) return norm_launch<DT, MODE, 1, 8>(p, stream);
