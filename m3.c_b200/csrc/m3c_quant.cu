@@ -62,7 +62,7 @@ unsigned capped_grid(uint64_t wanted, unsigned per_sm)
 // 16-bit residual stream.  16384 x 4096 bf16 with residual: 74.4 us, 6.3 TB/s,
 // 0.96 of the measured copy rate; in groups of 128, which make a divisor per
 // eight elements, 85.8 us (0.84).  Without a residual, three bytes an element,
-// the instructions (some twelve an element) weigh more: 52 us (0.59).  Both
+// the instructions weigh more: 52 us (0.59).  Both
 // kernels below read a row once and keep h on the SM until its codes are out.
 
 // The register kernel: `threads` threads (whole warps) own a row, each K pieces
@@ -569,9 +569,9 @@ int norm_mode(const m3c_norm_e4m3_params &p, bool vectors, cudaStream_t stream)
 
 // ------------------------------------------------------------------ cache
 
-// Where packed row t lies in the cache: its slot, or -1 where it has none (not
-// in a sequence, or skipped and recorded).  `s` is the last sequence that
-// begins at or before t, if any does.
+// Where packed row t lies in the cache: the number of its slot's first vector
+// (slot * heads), or -1 where it has none (not in a sequence, or skipped and
+// recorded).  `s` is the last sequence that begins at or before t, if any does.
 __device__ __forceinline__ int64_t slot_in_sequence(const m3c_cache_params &p, uint32_t t, uint32_t s)
 {
     const int64_t row = t;
@@ -585,7 +585,7 @@ __device__ __forceinline__ int64_t slot_in_sequence(const m3c_cache_params &p, u
         if (at < p.page_table_stride) {
             const int64_t page = p.page_table[s * p.page_table_stride + at];
             if (page >= 0 && static_cast<uint64_t>(page) < p.pages) {
-                return page * p.page_tokens + static_cast<int64_t>(static_cast<uint32_t>(position) - at * p.page_tokens);
+                return (page * p.page_tokens + (static_cast<uint32_t>(position) - at * p.page_tokens)) * p.heads;
             }
             reason = M3C_CACHE_BAD_PAGE;
         }
@@ -594,7 +594,7 @@ __device__ __forceinline__ int64_t slot_in_sequence(const m3c_cache_params &p, u
     return -1;
 }
 
-// The slots of `count` consecutive rows, by one warp: the sequence of the first
+// The slots (their first vectors) of `count` consecutive rows, by one warp: the sequence of the first
 // by a 32-way search (a step for 32 sequences, two for 1024), the others' from
 // there on.
 __device__ __forceinline__ void find_slots(const m3c_cache_params &p, uint32_t first, uint32_t count, int64_t *slots)
@@ -639,7 +639,7 @@ __device__ __forceinline__ void find_slots(const m3c_cache_params &p, uint32_t f
 // Bytes bound both directions: three per element of 16-bit rows.  262144 rows
 // of 8 heads of 128 in bf16 are read in 250 us (6.5 TB/s, 0.98 of the measured
 // copy rate), 65536 written in 74.5 us (5.5 TB/s, 0.83), 16384 in 21.1 us (0.73).
-// Writing has some eleven instructions an element (the maximum over the vector,
+// Writing has some twelve instructions an element (the maximum over the vector,
 // a correctly rounded quotient) and the dependent loads that find a slot.
 struct cache_shape {
     uint32_t lane_shift;
@@ -696,12 +696,16 @@ __global__ void __launch_bounds__(CACHE_THREADS, 2)
     bool inside[P];
 #pragma unroll
     for (int j = 0; j < P; ++j) inside[j] = at.owner && (j * at.lanes + at.lane) * 8u < p.head_dim;
+    // the thread's next row, and the way from row to row, in bytes
+    const char *row = base + at.side * token_stride * (DT == M3C_F32 ? 4u : 2u);
+    const uint64_t stride = shape.rows * token_stride * (DT == M3C_F32 ? 4u : 2u);
     auto load = [&](uint32_t r, Piece<DT, 8> (&piece)[P]) {
 #pragma unroll
         for (int j = 0; j < P; ++j) {
             piece[j] = {};
-            if (inside[j] && r < at.count) piece[j] = load_piece<DT, 8>(base, r * token_stride + j * at.lanes * 8u);
+            if (inside[j] && r < at.count) piece[j] = load_piece<DT, 8>(row, j * at.lanes * 8u);
         }
+        row += stride;
     };
     Piece<DT, 8> next[P];
     load(at.side, next);
@@ -727,7 +731,7 @@ __global__ void __launch_bounds__(CACHE_THREADS, 2)
         const int64_t slot = at.owner && r < at.count ? slots[r] : -1;
         if (slot >= 0) {
             const e4m3_divisor d = e4m3_divide_by(e4m3_scale(largest));
-            const uint64_t vector = static_cast<uint64_t>(slot) * p.heads + at.head;
+            const uint64_t vector = static_cast<uint64_t>(slot) + at.head;
             if (at.lane == 0u) scales[vector] = d.scale;
 #pragma unroll
             for (int j = 0; j < P; ++j) {
@@ -762,7 +766,7 @@ __global__ void __launch_bounds__(CACHE_THREADS)
     for (int i = 0; i < STEPS; ++i) {
         const uint32_t r = i * shape.rows + at.side;
         const int64_t slot = r < at.count ? slots[r] : -1;
-        const uint64_t vector = static_cast<uint64_t>(slot) * p.heads + at.head;
+        const uint64_t vector = static_cast<uint64_t>(slot) + at.head;
         live[i] = slot >= 0;
         scale[i] = live[i] ? p.scales[at.kv][vector] : 0.0f;
 #pragma unroll
@@ -806,7 +810,7 @@ __global__ void __launch_bounds__(QUANT_THREADS) cache_any_kernel(const __grid_c
         __syncwarp();
         const int64_t slot = slots[threadIdx.x / 32];
         if (slot < 0) continue;
-        const uint64_t at = static_cast<uint64_t>(slot) * p.heads + head;
+        const uint64_t at = static_cast<uint64_t>(slot) + head;
         const uint64_t row = t * p.token_stride[kv] + head * p.head_stride[kv];
         uint8_t *codes = p.codes[kv] + at * p.head_dim;
         if constexpr (WRITE) {
