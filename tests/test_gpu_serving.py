@@ -228,6 +228,56 @@ def test_norm_small_scales(m3, gpu):
         assert np.all((nearest_e4m3(q - reach) <= got) & (got <= nearest_e4m3(q + reach)))
 
 
+@pytest.mark.parametrize("width, group", [(60008, 60008), (60001, 60001), (60000, 30000), (52000, 8)])
+def test_norm_rows_past_shared_memory(m3, gpu, width, group):
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(width)
+    x, r = (torch.randn(5, width, generator=g, device="cuda").bfloat16() for _ in range(2))
+    w = torch.randn(width, generator=g, device="cuda")
+    h = (x.float() + r.float()).bfloat16()
+    check_norm(h, w, group, *run_norm(m3, x, w, group, r, None))
+    codes, scales = run_norm(m3, x, w, group, r, x)         # in place: read back as the sum
+    assert torch.equal(x, h)
+    check_norm(h, w, group, codes, scales)
+
+
+@pytest.mark.parametrize("shift", [0, 1, 4, 8])
+@pytest.mark.parametrize("width, group", [(256, 256), (256, 32), (2048, 256)])
+def test_norm_codes_at_any_address(m3, gpu, width, group, shift):
+    import torch
+
+    x = torch.randn(9, width, device="cuda").bfloat16()
+    w = torch.randn(width, device="cuda").bfloat16()
+    codes = torch.full((9 * width + 32,), 0x55, dtype=torch.uint8, device="cuda")
+    scales = torch.zeros(9 * (width // group) + 1, device="cuda")[1:]
+    m3.rms_norm_e4m3(m3.RmsNormE4m3Args(
+        input=x.data_ptr(), dtype=m3.BF16, scale=w.data_ptr(), scale_dtype=m3.BF16, rows=9, width=width, group=group,
+        codes=codes.data_ptr() + shift, code_scales=scales.data_ptr()))
+    torch.cuda.synchronize()
+    check_norm(x, w, group, codes[shift:shift + 9 * width].view(9, width), scales.view(9, -1))
+    assert bool((codes[:shift] == 0x55).all()) and bool((codes[shift + 9 * width:] == 0x55).all())
+
+
+def test_norm_past_32_bit_offsets(m3, gpu):
+    """More than 2^32 elements: the last rows."""
+    import torch
+
+    rows, width = 262200, 16384
+    assert rows * width > 1 << 32
+    x = torch.zeros(rows, width, dtype=torch.bfloat16, device="cuda")
+    x[-3:] = torch.randn(3, width, device="cuda").bfloat16()
+    w = torch.randn(width, device="cuda").bfloat16()
+    codes = torch.empty(rows, width, dtype=torch.uint8, device="cuda")
+    scales = torch.empty(rows, width // 128, device="cuda")
+    m3.rms_norm_e4m3(m3.RmsNormE4m3Args(
+        input=x.data_ptr(), dtype=m3.BF16, scale=w.data_ptr(), scale_dtype=m3.BF16, rows=rows, width=width, group=128,
+        codes=codes.data_ptr(), code_scales=scales.data_ptr()))
+    torch.cuda.synchronize()
+    check_norm(x[-3:], w, 128, codes[-3:], scales[-3:])
+    assert not bool((codes[-6:-3] & 0x7f).any()) and bool((scales[-6:-3] == TINY).all())
+
+
 def test_norm_zero_rows_and_repeat(m3, gpu):
     import torch
 
@@ -869,6 +919,25 @@ def test_verify_bad_sequences_stay_alone(m3, gpu):
     m3.verify_draft(m3.VerifyDraftArgs(batch=0, vocabulary=5))
 
 
+def test_verify_past_32_bit_offsets(m3, gpu):
+    """Rows of probabilities past 2^32 elements."""
+    import torch
+
+    batch, vocabulary = 16500, 131080
+    target = torch.zeros(batch, 2, vocabulary, dtype=torch.float16, device="cuda")
+    assert target.numel() > 1 << 32
+    g = torch.Generator(device="cuda").manual_seed(6)
+    target[-4:] = torch.softmax(torch.randn(4, 2, vocabulary, generator=g, device="cuda"), -1).half()
+    target[:-4, :, 77] = 1.0
+    drafted = torch.full((batch, 1), 77, dtype=torch.int32, device="cuda")
+    uniforms = torch.rand(batch, 2, generator=g, device="cuda")
+    uniforms[-2:, 0] = 0.0
+    tokens, accepted = run_verify(m3, target, None, drafted, None, uniforms)
+    want = verify_host(host(target[-4:]), None, drafted[-4:].cpu().numpy(), None, host(uniforms[-4:]))
+    assert np.array_equal(tokens[-4:], want[0]) and np.array_equal(accepted[-4:], want[1])
+    assert np.all(tokens[:-4] == 77) and np.all(accepted[:-4] == 1)
+
+
 def test_verify_distribution(m3, gpu):
     """The first token's frequencies are the target's, whatever the draft model."""
     import torch
@@ -1139,6 +1208,41 @@ def test_verify_behind_softmax_in_a_session(m3, gpu, drawn, ragged):
     want = verify_host(target, q.astype(np.float64) if drawn else None, tokens, lengths if ragged else None,
                        uniforms.astype(np.float64) / 2)
     assert np.array_equal(s.read(out), want[0]) and np.array_equal(s.read(accepted), want[1])
+
+
+def test_serving_operators_beside_others_in_a_wave(m3, gpu):
+    """Independent launches without a data check run at the same time."""
+    import torch
+
+    g = m3.Graph()
+    x, w = g.value(m3.INPUT, m3.BF16, (512, 1024)), g.value(m3.INPUT, m3.F32, (1024,))
+    codes = g.inferred("RMS_NORM_E4M3", [x, w], m3.OUTPUT, m3.E4M3, epsilon=1e-6)
+    scales = g.inferred("RMS_NORM_E4M3", [x, w], m3.OUTPUT, m3.F32, 1, epsilon=1e-6)
+    g.node("RMS_NORM_E4M3", [x, w], [codes, scales], epsilon=1e-6)
+    target, tokens = g.value(m3.INPUT, m3.F32, (8, 3, 4000)), g.value(m3.INPUT, m3.I32, (8, 2))
+    uniforms = g.value(m3.INPUT, m3.F32, (8, 3))
+    out = g.inferred("VERIFY_DRAFT", [target, tokens, uniforms], m3.OUTPUT, m3.I32, 0)
+    accepted = g.inferred("VERIFY_DRAFT", [target, tokens, uniforms], m3.OUTPUT, m3.I32, 1)
+    g.node("VERIFY_DRAFT", [target, tokens, uniforms], [out, accepted])
+    a = g.value(m3.INPUT, m3.F32, (4096, 512))
+    doubled = g.inferred("ADD", [a, a], m3.OUTPUT, m3.F32)
+    g.node("ADD", [a, a], [doubled])
+    rng = np.random.default_rng(12)
+    s = m3.Session(g)
+    hx = torch.from_numpy(rng.normal(size=(512, 1024))).bfloat16()
+    hw = rng.normal(size=1024).astype(np.float32)
+    ht = rng.dirichlet(np.ones(4000) * 0.05, (8, 3)).astype(np.float32)
+    hk, hu = ht[:, :2].argmax(-1).astype(np.int32), rng.uniform(0, 0.2, (8, 3)).astype(np.float32)
+    ha = rng.normal(size=(4096, 512)).astype(np.float32)
+    for value, data in ((x, raw(hx)), (w, hw), (target, ht), (tokens, hk), (uniforms, hu), (a, ha)):
+        s.write(value, data)
+    for _ in range(5):
+        s.run_async()
+    s.synchronize()
+    check_norm(hx, torch.from_numpy(hw), 1024, torch.from_numpy(s.read(codes)), torch.from_numpy(s.read(scales)))
+    want = verify_host(ht.astype(np.float64), None, hk, None, hu.astype(np.float64))
+    assert np.array_equal(s.read(out), want[0]) and np.array_equal(s.read(accepted), want[1])
+    assert np.array_equal(s.read(doubled), ha + ha)
 
 
 def test_empty_batches_in_a_session(m3, gpu):
