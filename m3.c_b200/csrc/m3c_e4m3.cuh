@@ -24,7 +24,9 @@ constexpr float E4M3_SMALLEST_SCALE = 0x1p-126f;
 // div_markstein's remainder v - q s is a multiple of ulp(q) ulp(s).  Quotients
 // below 2^-10 have the code 0 however they round, and for the others the
 // remainder is exact while 2^-33 * 2^-23 s >= 2^-149.
+// Smaller scales and their values are lifted first, which is exact.
 constexpr float E4M3_MARKSTEIN_SCALE = 0x1p-90f;
+constexpr float E4M3_LIFT = 0x1p64f;
 
 // The magnitude as an integer: ordered like |v|, with NaN above infinity, so a
 // maximum of these keeps a NaN that a float maximum would drop.
@@ -37,31 +39,25 @@ __device__ __forceinline__ float e4m3_scale(uint32_t largest_bits)
 {
     if (largest_bits >= 0x7f800000u) return as_float(0x7fc00000u);
     const float a = as_float(largest_bits);
-    const float s = a < E4M3_MARKSTEIN_SCALE ? __fdiv_rn(a, E4M3_LARGEST)
-                                             : div_markstein(a, E4M3_LARGEST, E4M3_LARGEST_RECIPROCAL);
-    return fmaxf(s, E4M3_SMALLEST_SCALE);
+    const float lift = a < E4M3_MARKSTEIN_SCALE ? E4M3_LIFT : 1.0f;
+    const float s = div_markstein(__fmul_rn(a, lift), E4M3_LARGEST, E4M3_LARGEST_RECIPROCAL);
+    return fmaxf(lift == 1.0f ? s : __fmul_rn(s, 1.0f / E4M3_LIFT), E4M3_SMALLEST_SCALE);
 }
 
-// The divisor of one group: its scale and the scale's rounded reciprocal, or a
-// reciprocal of 0 where the scale is too small for div_markstein.
+// The divisor of one group: its scale, lifted by a power of two with the values
+// where it is too small for div_markstein, and that number's rounded reciprocal.
 struct e4m3_divisor {
     float scale;
+    float lift;
+    float lifted;
     float reciprocal;
 };
 
 __device__ __forceinline__ e4m3_divisor e4m3_divide_by(float scale)
 {
-    return {scale, scale < E4M3_MARKSTEIN_SCALE ? 0.0f : __frcp_rn(scale)};
-}
-
-__device__ __forceinline__ float e4m3_quotient(float v, const e4m3_divisor &d)
-{
-    return d.reciprocal == 0.0f ? __fdiv_rn(v, d.scale) : div_markstein(v, d.scale, d.reciprocal);
-}
-
-__device__ __forceinline__ uint8_t e4m3_code(float v, const e4m3_divisor &d)
-{
-    return __nv_cvt_float_to_fp8(e4m3_quotient(v, d), __NV_SATFINITE, __NV_E4M3);
+    const float lift = scale < E4M3_MARKSTEIN_SCALE ? E4M3_LIFT : 1.0f;
+    const float lifted = __fmul_rn(scale, lift);
+    return {scale, lift, lifted, __frcp_rn(lifted)};
 }
 
 // The largest magnitude of N values, a NaN if one of them is a NaN.
@@ -93,33 +89,26 @@ __device__ __forceinline__ uint32_t e4m3_four(const float *q)
     return codes;
 }
 
-// Store the codes of eight values (to an 8-byte boundary) or of one.
+// Store the codes of eight values (to an 8-byte boundary) or of one: quotients by
+// div_markstein's steps, two a packed instruction.
 template <int N>
 __device__ __forceinline__ void e4m3_store(uint8_t *to, const float (&v)[N], const e4m3_divisor &d)
 {
     static_assert(N == 1 || N == 8, "one code or eight");
-    float q[N];
-    if (d.reciprocal == 0.0f) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) q[i] = __fdiv_rn(v[i], d.scale);
-    } else {
-        // div_markstein, two quotients a packed instruction
-        if constexpr (N == 1) {
-            q[0] = div_markstein(v[0], d.scale, d.reciprocal);
-        } else {
-            const uint64_t y = f2_splat(d.reciprocal);
-            const uint64_t s = f2_splat(-d.scale);
-#pragma unroll
-            for (int i = 0; i < N; i += 2) {
-                const uint64_t a = f2_pack(v[i], v[i + 1]);
-                const uint64_t q0 = f2_mul(a, y);
-                f2_unpack(f2_fma(f2_fma(q0, s, a), y, q0), q[i], q[i + 1]);
-            }
-        }
-    }
     if constexpr (N == 1) {
-        *to = __nv_cvt_float_to_fp8(q[0], __NV_SATFINITE, __NV_E4M3);
+        *to = __nv_cvt_float_to_fp8(div_markstein(__fmul_rn(v[0], d.lift), d.lifted, d.reciprocal), __NV_SATFINITE,
+                                    __NV_E4M3);
     } else {
+        float q[N];
+        const uint64_t y = f2_splat(d.reciprocal);
+        const uint64_t s = f2_splat(-d.lifted);
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            uint64_t a = f2_pack(v[i], v[i + 1]);
+            if (d.lift != 1.0f) a = f2_mul(a, f2_splat(d.lift));
+            const uint64_t q0 = f2_mul(a, y);
+            f2_unpack(f2_fma(f2_fma(q0, s, a), y, q0), q[i], q[i + 1]);
+        }
         *reinterpret_cast<uint2 *>(to) = make_uint2(e4m3_four(q), e4m3_four(q + 4));
     }
 }

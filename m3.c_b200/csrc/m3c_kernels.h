@@ -236,7 +236,7 @@ typedef struct {
     uint32_t skip_before;       /* session launches: as in m3c_norm_params */
     m3c_status *status;         /* NULL: a direct call */
     int32_t first_of_run;
-    int32_t reserved;
+    float width_reciprocal;     /* set by the launch */
 } m3c_norm_e4m3_params;
 
 int m3c_launch_norm_e4m3(const m3c_norm_e4m3_params *params, void *stream);

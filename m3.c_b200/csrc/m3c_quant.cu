@@ -59,10 +59,10 @@ unsigned capped_grid(uint64_t wanted, unsigned per_sm)
 //   per group of y: scale, codes (m3c_e4m3.cuh).
 //
 // Bytes bound it: x and r in, h and the codes out, 7 bytes per element of a
-// 16-bit residual stream.  16384 x 4096 bf16 with residual: 74.4 us, 6.3 TB/s,
-// 0.96 of the measured copy rate; in groups of 128, which make a divisor per
-// eight elements, 85.8 us (0.84).  Without a residual, three bytes an element,
-// the instructions weigh more: 52 us (0.59).  Both
+// 16-bit residual stream.  16384 x 4096 bf16 with residual: 73.5 us, 6.4 TB/s,
+// 0.97 of the measured copy rate; in groups of 128, which make a divisor per
+// eight elements, 85.2 us (0.84).  Without a residual, three bytes an element,
+// the instructions weigh more: 46.3 us (0.66).  Both
 // kernels below read a row once and keep h on the SM until its codes are out.
 
 // The register kernel: `threads` threads (whole warps) own a row, each K pieces
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(norm_block(VEC, K))
         if constexpr (MODE == GROUP_ROW) largest = warp_max(lane < warps ? top[first + lane] : 0u);
     }
     if (!live) return;
-    const float inverse = __frsqrt_rn(__fadd_rn(__fdiv_rn(squares[0], static_cast<float>(width)), p.epsilon));
+    const float inverse = __frsqrt_rn(__fadd_rn(__fmul_rn(squares[0], p.width_reciprocal), p.epsilon));
     norm_divisor d;
     if constexpr (MODE == GROUP_ROW) {
         d = divide_norm_by(as_float(largest), inverse);
@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(QUANT_THREADS)
         squares = 0.0f;
         for (int w = 0; w < QUANT_WARPS; ++w) squares = __fadd_rn(squares, part[w]);
         const float inverse =
-            __frsqrt_rn(__fadd_rn(__fdiv_rn(squares, static_cast<float>(p.width)), p.epsilon));
+            __frsqrt_rn(__fadd_rn(__fmul_rn(squares, p.width_reciprocal), p.epsilon));
         auto weighted = [&](uint64_t j) {
             // the stored sum is h (and may be the input's own storage by now)
             const float h = kept                   ? held[j]
@@ -508,8 +508,9 @@ __global__ void __launch_bounds__(QUANT_THREADS)
             const norm_divisor d = divide_norm_by(as_float(largest), inverse);
             if (from == 0) p.code_scales[row * groups + g] = d.scale;
             for (uint64_t j = from; j < p.group; j += step) {
-                const float z = weighted(g0 + j);
-                codes[g0 + j] = e4m3_code(d.normed ? __fmul_rn(z, inverse) : z, d.by);
+                float z[1] = {weighted(g0 + j)};
+                if (d.normed) multiply(z, inverse);
+                e4m3_store<1>(codes + g0 + j, z, d.by);
             }
             if (!alone) __syncthreads();
         }
@@ -545,7 +546,7 @@ int norm_depth(const m3c_norm_e4m3_params &p, bool vectors, cudaStream_t stream)
     if (!vectors) return norm_launch<DT, MODE, 1, 8>(p, stream);
     // pieces per thread.  What a thread does once per row (the root, the
     // divisor) weighs on two pieces: many rows of one group take four (16384 x
-    // 4096 bf16 without residual: 52 us against 57).  With a divisor per
+    // 4096 bf16 without residual: a tenth less time).  With a divisor per
     // piece, or too few rows to fill the SMs with a row's fewer threads, two
     // are faster (the same rows in groups of 128: 86 us against 90), as with
     // F32's wider pieces (8192 x 4096 with residual: 70 us against 72).  Rows
@@ -822,7 +823,8 @@ __global__ void __launch_bounds__(QUANT_THREADS) cache_any_kernel(const __grid_c
             const e4m3_divisor d = e4m3_divide_by(e4m3_scale(warp_max(largest)));
             if (lane == 0) p.scales[kv][at] = d.scale;
             for (uint32_t j = lane; j < p.head_dim; j += 32) {
-                codes[j] = e4m3_code(load_element(p.rows[kv], p.dtype[kv], row + j), d);
+                const float v[1] = {load_element(p.rows[kv], p.dtype[kv], row + j)};
+                e4m3_store<1>(codes + j, v, d);
             }
         } else {
             const float scale = p.scales[kv][at];
@@ -932,7 +934,8 @@ int launch_cache(const m3c_cache_params &p, cudaStream_t stream)
 extern "C" int m3c_launch_norm_e4m3(const m3c_norm_e4m3_params *params, void *stream)
 {
     using namespace m3c;
-    const m3c_norm_e4m3_params &p = *params;
+    m3c_norm_e4m3_params p = *params;
+    p.width_reciprocal = 1.0f / static_cast<float>(p.width);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const uint64_t step = p.dtype == M3C_F32 ? 4u : 8u;  // elements of 16 bytes
     const bool vectors = p.width % 8u == 0u && p.group % 8u == 0u && p.x_stride % step == 0u && aligned_to(p.x, 16) &&
