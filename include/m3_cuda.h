@@ -987,6 +987,8 @@ typedef struct {
     uint32_t head_dim;
 } m3_cuda_cache_options;
 
+/* The current device, pages of 16 tokens; the rest is the caller's (zero). */
+void m3_cuda_cache_options_init(m3_cuda_cache_options *options);
 m3_status m3_cuda_cache_create(m3_cuda_cache **cache,
                                const m3_cuda_cache_options *options,
                                m3_error *error);

@@ -266,6 +266,15 @@ m3_status m3_cuda_rms_norm_e4m3(int device, void *stream,
 #define CACHE_CLEAN (~0ULL)
 #define CACHE_PART_LIMIT ((uint64_t)1 << 20)
 
+void m3_cuda_cache_options_init(m3_cuda_cache_options *options)
+{
+    if (options != NULL) {
+        memset(options, 0, sizeof(*options));
+        options->device = M3_CUDA_DEVICE_CURRENT;
+        options->page_tokens = 16U;
+    }
+}
+
 static uint64_t align_up(uint64_t bytes)
 {
     return (bytes + M3C_ARENA_ALIGNMENT - 1U) &

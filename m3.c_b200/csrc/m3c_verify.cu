@@ -10,11 +10,13 @@
 // rounding errors of a sum past whole tokens' probabilities.
 //
 // Bytes bound large batches (one row of each model per sequence), latency small
-// ones.  A cluster of CTAs takes a sequence, its warps one contiguous part of
-// the vocabulary each.  One pass over the rows sums the parts; the parts' sums
-// go round through the CTAs' shared memory, and the CTA that owns the part in
-// which the running sum passes the aim looks for the token there, in a part
-// of a few KB that is still in the L2.
+// ones: 128 sequences over 131072 tokens in F32 take 28.7 us (4.7 TB/s, 0.71 of
+// the measured copy rate), one over 32000 takes 6.5 us, nearly all of it loads
+// that wait for one another.  A cluster of CTAs takes a sequence, its warps one
+// contiguous part of the vocabulary each.  One pass over the rows sums the
+// parts; the parts' sums go round through the CTAs' shared memory, and the CTA
+// that owns the part in which the running sum passes the aim looks for the token
+// there, in a few KB that are still in the L2.
 
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -151,9 +153,10 @@ __device__ __forceinline__ double weight(float t, float q)
 // q and what its rounding lost, which F32 holds exactly (T. J. Dekker, "A
 // floating-point technique for extending the available precision", Numer. Math.
 // 18, 1971: |max(t, q)| >= |q|).  The d are summed in 64 bits, with one
-// conversion each instead of two; what was lost is below 2^-24 of that, so its
-// own sum in F32 adds an error below 2^-40 of the smallest difference that the
-// running sums make.
+// conversion each instead of two; what was lost is below 2^-24 of that, and its
+// own sum, a few hundred F32 additions a lane, is off by less than 2^-40 of the
+// total: far below a token's weight, so the drawn token is that of a 64-bit sum
+// but for borders nearer than that.
 struct running_sum {
     double high = 0.0;
     float low = 0.0f;

@@ -467,6 +467,7 @@ _CUDA_SIGNATURES = {
     "m3_cuda_verify_draft": (ctypes.c_int, [
         ctypes.c_int, ctypes.c_void_p, ctypes.POINTER(VerifyDraftArgs),
         ctypes.POINTER(M3Error)]),
+    "m3_cuda_cache_options_init": (None, [ctypes.POINTER(CacheOptions)]),
     "m3_cuda_cache_create": (ctypes.c_int, [
         ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(CacheOptions),
         ctypes.POINTER(M3Error)]),

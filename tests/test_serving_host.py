@@ -79,6 +79,11 @@ def test_initialisers(m3):
     m3.load().m3_cuda_verify_draft_args_init(verify)
     assert norm.rows == 0 and abs(norm.epsilon - 1e-6) < 1e-12 and not norm.input
     assert verify.batch == 0 and not verify.target
+    cache = m3.CacheOptions(5, 5, 5, 5, 5)
+    m3.load().m3_cuda_cache_options_init(cache)
+    assert (cache.device, cache.pages, cache.page_tokens, cache.heads, cache.head_dim) == (-1, 0, 16, 0, 0)
+    for init in ("rms_norm_e4m3_args", "verify_draft_args", "cache_options"):
+        getattr(m3.load(), f"m3_cuda_{init}_init")(None)
 
 
 def verify_args(m3, **change):
