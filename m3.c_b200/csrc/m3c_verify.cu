@@ -153,10 +153,9 @@ __device__ __forceinline__ double weight(float t, float q)
 // q and what its rounding lost, which F32 holds exactly (T. J. Dekker, "A
 // floating-point technique for extending the available precision", Numer. Math.
 // 18, 1971: |max(t, q)| >= |q|).  The d are summed in 64 bits, with one
-// conversion each instead of two; what was lost is below 2^-24 of that, and its
-// own sum, a few hundred F32 additions a lane, is off by less than 2^-40 of the
-// total: far below a token's weight, so the drawn token is that of a 64-bit sum
-// but for borders nearer than that.
+// conversion each instead of two; what was lost is below 2^-24 of that, and is
+// summed in F32 for some eight numbers before it joins them, off by less than
+// 2^-45 of their sum.
 struct running_sum {
     double high = 0.0;
     float low = 0.0f;
@@ -169,7 +168,11 @@ struct running_sum {
         high += static_cast<double>(d);
     }
 
-    __device__ __forceinline__ double value() const { return high + static_cast<double>(low); }
+    __device__ __forceinline__ void join()
+    {
+        high += static_cast<double>(low);
+        low = 0.0f;
+    }
 };
 
 __device__ __forceinline__ double shuffle_up(double v, int d)
@@ -264,6 +267,8 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 1024 / VERIFY_THREADS)
                 }
 #pragma unroll
                 for (int l = 0; l < LOADS; ++l) add(j + l * 32u * VEC, target[l], draft[l]);
+                run[0].join();
+                run[1].join();
             }
             for (; j + VEC <= end; j += 32u * VEC) {
                 Stored<DT, VEC> target;
@@ -278,7 +283,9 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 1024 / VERIFY_THREADS)
                 largest = largest_word(largest_word(largest, t), q);
                 run[0].add(j == from.given ? 0.0f : t[0], q[0]);
             }
-            double sum = run[0].value() + run[1].value();
+            run[0].join();
+            run[1].join();
+            double sum = run[0].high + run[1].high;
             const bool valid = largest < 0x7f800000u;
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
