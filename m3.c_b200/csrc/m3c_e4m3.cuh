@@ -89,12 +89,12 @@ __device__ __forceinline__ uint32_t e4m3_four(const float *q)
     return codes;
 }
 
-// Store the codes of eight values (to an 8-byte boundary) or of one: quotients by
-// div_markstein's steps, two a packed instruction.
+// Store the codes of 16 or eight values (to a boundary of as many bytes) or of
+// one: quotients by div_markstein's steps, two a packed instruction.
 template <int N>
 __device__ __forceinline__ void e4m3_store(uint8_t *to, const float (&v)[N], const e4m3_divisor &d)
 {
-    static_assert(N == 1 || N == 8, "one code or eight");
+    static_assert(N == 1 || N == 8 || N == 16, "one code, eight or 16");
     if constexpr (N == 1) {
         *to = __nv_cvt_float_to_fp8(div_markstein(__fmul_rn(v[0], d.lift), d.lifted, d.reciprocal), __NV_SATFINITE,
                                     __NV_E4M3);
@@ -109,7 +109,12 @@ __device__ __forceinline__ void e4m3_store(uint8_t *to, const float (&v)[N], con
             const uint64_t q0 = f2_mul(a, y);
             f2_unpack(f2_fma(f2_fma(q0, s, a), y, q0), q[i], q[i + 1]);
         }
-        *reinterpret_cast<uint2 *>(to) = make_uint2(e4m3_four(q), e4m3_four(q + 4));
+        if constexpr (N == 16) {
+            *reinterpret_cast<uint4 *>(to) =
+                make_uint4(e4m3_four(q), e4m3_four(q + 4), e4m3_four(q + 8), e4m3_four(q + 12));
+        } else {
+            *reinterpret_cast<uint2 *>(to) = make_uint2(e4m3_four(q), e4m3_four(q + 4));
+        }
     }
 }
 

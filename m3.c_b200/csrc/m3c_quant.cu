@@ -18,6 +18,9 @@ constexpr int QUANT_THREADS = 256;
 constexpr int QUANT_WARPS = QUANT_THREADS / 32;
 constexpr int NORM_THREADS = 128;                   // rows share a CTA up to these
 constexpr uint64_t NORM_WIDEST = 16384;             // of the register kernel
+#ifndef NV16MIN
+#define NV16MIN 16u
+#endif
 constexpr uint64_t NORM_KEPT_BYTES = 200u * 1024u;  // of shared memory for a row
 
 __device__ __forceinline__ float warp_sum(float v)
@@ -97,6 +100,12 @@ __device__ __forceinline__ Piece<DT, VEC> load_piece(const void *base, uint64_t 
         v.w[0] = __ldcs(reinterpret_cast<const unsigned short *>(from));
     } else if constexpr (Piece<DT, VEC>::BYTES == 4) {
         v.w[0] = __ldcs(reinterpret_cast<const unsigned *>(from));
+    } else if constexpr (Piece<DT, VEC>::BYTES == 32 && VEC == 16) {
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]),
+                       "=r"(v.w[6]), "=r"(v.w[7])
+                     : "l"(from)
+                     : "memory");
     } else {
 #pragma unroll
         for (int i = 0; i < Piece<DT, VEC>::WORDS / 4; ++i) {
@@ -120,7 +129,7 @@ __device__ __forceinline__ void store_piece(void *base, uint64_t element, const 
         *reinterpret_cast<uint16_t *>(to) = static_cast<uint16_t>(v.w[0]);
     } else if constexpr (Piece<DT, VEC>::BYTES == 4) {
         *reinterpret_cast<uint32_t *>(to) = v.w[0];
-    } else if constexpr (Piece<DT, VEC>::BYTES == 32 && WIDE) {
+    } else if constexpr (Piece<DT, VEC>::BYTES == 32 && (WIDE || VEC == 16)) {
         asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v.w[0]), "r"(v.w[1]),
                      "r"(v.w[2]), "r"(v.w[3]), "r"(v.w[4]), "r"(v.w[5]), "r"(v.w[6]), "r"(v.w[7])
                      : "memory");
@@ -205,8 +214,8 @@ __device__ __forceinline__ void add_piece(Piece<DT, VEC> &a, const Piece<DT, VEC
 }
 
 // VEC weights; the same for every row, they stay in the caches.  They are read
-// with the row, but for eight F32 ones, which take twice the registers and are
-// read when used.
+// with the row, but for eight or more F32 ones, which take twice the registers
+// and are read when used.
 template <int VEC>
 struct Weights {
     Piece<M3C_F16, VEC> early;
@@ -216,9 +225,12 @@ struct Weights {
         const uint16_t *from = static_cast<const uint16_t *>(scale) + element;
         if (dtype == M3C_F32) {
             if constexpr (VEC == 1) early.w[0] = __ldg(static_cast<const uint32_t *>(scale) + element);
-        } else if constexpr (VEC == 8) {
-            const uint4 q = __ldg(reinterpret_cast<const uint4 *>(from));
-            early.w[0] = q.x, early.w[1] = q.y, early.w[2] = q.z, early.w[3] = q.w;
+        } else if constexpr (VEC >= 8) {
+#pragma unroll
+            for (int i = 0; i < VEC / 8; ++i) {
+                const uint4 q = __ldg(reinterpret_cast<const uint4 *>(from) + i);
+                early.w[4 * i] = q.x, early.w[4 * i + 1] = q.y, early.w[4 * i + 2] = q.z, early.w[4 * i + 3] = q.w;
+            }
         } else {
             early.w[0] = __ldg(from);
         }
@@ -228,11 +240,12 @@ struct Weights {
     {
         if (dtype == M3C_F32) {
             const float *from = static_cast<const float *>(scale) + element;
-            if constexpr (VEC == 8) {
-                const float4 a = __ldg(reinterpret_cast<const float4 *>(from));
-                const float4 b = __ldg(reinterpret_cast<const float4 *>(from) + 1);
-                x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-                x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+            if constexpr (VEC >= 8) {
+#pragma unroll
+                for (int i = 0; i < VEC / 4; ++i) {
+                    const float4 a = __ldg(reinterpret_cast<const float4 *>(from) + i);
+                    x[4 * i] = a.x, x[4 * i + 1] = a.y, x[4 * i + 2] = a.z, x[4 * i + 3] = a.w;
+                }
             } else {
                 x[0] = as_float(early.w[0]);
             }
@@ -296,7 +309,7 @@ __device__ __forceinline__ norm_divisor divide_norm_by(float most, float inverse
 // The most threads of a CTA of the register kernel, as norm_depth chooses K.
 constexpr int norm_block(int vec, int k)
 {
-    return vec == 1 ? 1024 : k == 1 ? NORM_THREADS : k == 2 ? 512 : 256;
+    return vec == 1 ? 1024 : vec == 16 ? (k == 4 ? 256 : 512) : k == 1 ? NORM_THREADS : k == 2 ? 512 : 256;
 }
 
 template <int DT, int MODE, int VEC, int K>
@@ -538,8 +551,17 @@ int norm_launch(const m3c_norm_e4m3_params &p, cudaStream_t stream)
 }
 
 template <int DT, int MODE>
-int norm_depth(const m3c_norm_e4m3_params &p, bool vectors, cudaStream_t stream)
+int norm_depth(const m3c_norm_e4m3_params &p, bool vectors, bool wide, cudaStream_t stream)
 {
+    if constexpr (DT != M3C_F32) {
+        const uint64_t pieces = p.width / 16u;
+        const bool many = p.rows >= 2048u && MODE == GROUP_ROW;
+        if (wide && pieces > NV16MIN) {
+            if (pieces <= 512u && !(many && pieces > 32u)) return norm_launch<DT, MODE, 16, 1>(p, stream);
+            if (pieces <= 512u) return norm_launch<DT, MODE, 16, 2>(p, stream);
+            return norm_launch<DT, MODE, 16, 4>(p, stream);
+        }
+    }
     // single elements: 333 rows of 2051 F32 take 5.4 us with four per thread and
     // 6.4 with eight, which are for the widths that four leave past 1024 threads
     if (!vectors && p.width <= 4096u) return norm_launch<DT, MODE, 1, 4>(p, stream);
@@ -560,12 +582,12 @@ int norm_depth(const m3c_norm_e4m3_params &p, bool vectors, cudaStream_t stream)
 }
 
 template <int DT>
-int norm_mode(const m3c_norm_e4m3_params &p, bool vectors, cudaStream_t stream)
+int norm_mode(const m3c_norm_e4m3_params &p, bool vectors, bool wide, cudaStream_t stream)
 {
-    if (p.group == p.width) return norm_depth<DT, GROUP_ROW>(p, vectors, stream);
-    const uint64_t lanes = vectors ? p.group / 8u : p.group;
-    if (lanes <= 32u && (lanes & (lanes - 1)) == 0u) return norm_depth<DT, GROUP_LANES>(p, vectors, stream);
-    return norm_depth<DT, GROUP_WORDS>(p, vectors, stream);
+    const uint64_t lanes = p.group / (wide ? 16u : vectors ? 8u : 1u);
+    if (p.group == p.width) return norm_depth<DT, GROUP_ROW>(p, vectors, wide, stream);
+    if (lanes <= 32u && (lanes & (lanes - 1)) == 0u) return norm_depth<DT, GROUP_LANES>(p, vectors, wide, stream);
+    return norm_depth<DT, GROUP_WORDS>(p, vectors, wide, stream);
 }
 
 // ------------------------------------------------------------------ cache
@@ -942,11 +964,16 @@ extern "C" int m3c_launch_norm_e4m3(const m3c_norm_e4m3_params *params, void *st
                          aligned_to(p.scale, 16) && aligned_to(p.codes, 8) &&
                          (p.resid_b == nullptr || (p.resid_stride % step == 0u && aligned_to(p.resid_b, 16))) &&
                          (p.sum_out == nullptr || (p.sum_stride % step == 0u && aligned_to(p.sum_out, 16)));
+    const bool wide = vectors && p.dtype != M3C_F32 && p.width % 16u == 0u && p.group % 16u == 0u &&
+                      p.x_stride % 16u == 0u && aligned_to(p.x, 32) && aligned_to(p.codes, 16) &&
+                      (p.resid_b == nullptr || (p.resid_stride % 16u == 0u && aligned_to(p.resid_b, 32))) &&
+                      (p.sum_out == nullptr || (p.sum_stride % 16u == 0u && aligned_to(p.sum_out, 32))) &&
+                      p.width > 16u * NV16MIN;
     if (p.width <= (vectors ? NORM_WIDEST : NORM_WIDEST / 2u)) {
         switch (p.dtype) {
-        case M3C_F16: return norm_mode<M3C_F16>(p, vectors, s);
-        case M3C_BF16: return norm_mode<M3C_BF16>(p, vectors, s);
-        default: return norm_mode<M3C_F32>(p, vectors, s);
+        case M3C_F16: return norm_mode<M3C_F16>(p, vectors, wide, s);
+        case M3C_BF16: return norm_mode<M3C_BF16>(p, vectors, wide, s);
+        default: return norm_mode<M3C_F32>(p, vectors, wide, s);
         }
     }
     const size_t row_bytes = p.width * sizeof(float);
