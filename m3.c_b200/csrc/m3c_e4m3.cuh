@@ -123,19 +123,34 @@ __device__ __forceinline__ float e4m3_value(uint8_t code)
     return __half2float(__half(__nv_cvt_fp8_to_halfraw(code, __NV_E4M3)));
 }
 
-// The values of eight codes, exact.
-__device__ __forceinline__ void e4m3_values(const uint2 &codes, float (&x)[8])
-{
-    const uint32_t w[2] = {codes.x, codes.y};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __half2_raw two = __nv_cvt_fp8x2_to_halfraw2(
-            static_cast<__nv_fp8x2_storage_t>(w[i / 2] >> (i % 2 * 16)), __NV_E4M3);
-        const float2 f = __half22float2(__half2(two));
-        x[2 * i] = f.x;
-        x[2 * i + 1] = f.y;
+// N codes (eight or 16, at a boundary of as many bytes) and their exact values.
+template <int N>
+struct e4m3_codes {
+    uint32_t w[N / 4];
+
+    __device__ __forceinline__ void load(const uint8_t *from)
+    {
+        if constexpr (N == 16) {
+            const uint4 q = __ldcs(reinterpret_cast<const uint4 *>(from));
+            w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+        } else {
+            const uint2 q = __ldcs(reinterpret_cast<const uint2 *>(from));
+            w[0] = q.x, w[1] = q.y;
+        }
     }
-}
+
+    __device__ __forceinline__ void values(float (&x)[N]) const
+    {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            const __half2_raw two = __nv_cvt_fp8x2_to_halfraw2(
+                static_cast<__nv_fp8x2_storage_t>(w[i / 2] >> (i % 2 * 16)), __NV_E4M3);
+            const float2 f = __half22float2(__half2(two));
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
+    }
+};
 
 // Element i of a float tensor, and its store.
 __device__ __forceinline__ float load_element(const void *base, int dtype, uint64_t i)

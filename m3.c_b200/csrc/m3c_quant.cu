@@ -18,9 +18,6 @@ constexpr int QUANT_THREADS = 256;
 constexpr int QUANT_WARPS = QUANT_THREADS / 32;
 constexpr int NORM_THREADS = 128;                   // rows share a CTA up to these
 constexpr uint64_t NORM_WIDEST = 16384;             // of the register kernel
-#ifndef NV16MIN
-#define NV16MIN 16u
-#endif
 constexpr uint64_t NORM_KEPT_BYTES = 200u * 1024u;  // of shared memory for a row
 
 __device__ __forceinline__ float warp_sum(float v)
@@ -62,17 +59,18 @@ unsigned capped_grid(uint64_t wanted, unsigned per_sm)
 //   per group of y: scale, codes (m3c_e4m3.cuh).
 //
 // Bytes bound it: x and r in, h and the codes out, 7 bytes per element of a
-// 16-bit residual stream.  16384 x 4096 bf16 with residual: 73.5 us, 6.4 TB/s,
-// 0.97 of the measured copy rate; in groups of 128, which make a divisor per
-// eight elements, 85.2 us (0.84).  Without a residual, three bytes an element,
-// the instructions weigh more: 46.3 us (0.66).  Both
+// 16-bit residual stream.  16384 x 4096 bf16 with residual: 69.8 us, 6.7 TB/s,
+// 1.02 of the measured copy rate, in groups of 128 too; with accesses of 16 bytes
+// 73.5 us, and 85.2 in groups, which then made a divisor per eight elements.
+// Without a residual, three bytes an element, the instructions weigh more: 44.4
+// us (0.69).  Both
 // kernels below read a row once and keep h on the SM until its codes are out.
 
 // The register kernel: `threads` threads (whole warps) own a row, each K pieces
 // of VEC consecutive elements in registers, piece k of thread i being number
-// k * threads + i of the row, so a warp reads consecutive memory: VEC = 8 (16
-// bytes of a 16-bit row a lane) where every row is aligned for it, VEC = 1
-// elsewhere.  z = h w is made before the row's sum is known, and the largest |y|
+// k * threads + i of the row, so a warp reads consecutive memory: 32 bytes a lane
+// where every row is aligned for it (VEC = 16 elements of 16 bits, 8 of F32), 16
+// bytes (VEC = 8) or one element (VEC = 1) elsewhere.  z = h w is made before the row's sum is known, and the largest |y|
 // is the largest |z| times the inverse root (rounding keeps order), so one
 // exchange between a row's warps carries the sum of squares and the maximum.
 //   GROUP_ROW    one group per row
@@ -83,7 +81,8 @@ unsigned capped_grid(uint64_t wanted, unsigned per_sm)
 enum { GROUP_ROW, GROUP_LANES, GROUP_WORDS };
 
 // VEC elements as they are stored: h is a stored value already, so 16-bit rows
-// stay packed.
+// stay packed.  A piece of 32 bytes is read and written by one access, to a
+// 32-byte boundary: a sector at once.
 template <int DT, int VEC>
 struct Piece {
     static constexpr int BYTES = VEC * (DT == M3C_F32 ? 4 : 2);
@@ -100,7 +99,7 @@ __device__ __forceinline__ Piece<DT, VEC> load_piece(const void *base, uint64_t 
         v.w[0] = __ldcs(reinterpret_cast<const unsigned short *>(from));
     } else if constexpr (Piece<DT, VEC>::BYTES == 4) {
         v.w[0] = __ldcs(reinterpret_cast<const unsigned *>(from));
-    } else if constexpr (Piece<DT, VEC>::BYTES == 32 && VEC == 16) {
+    } else if constexpr (Piece<DT, VEC>::BYTES == 32) {
         asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                      : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]),
                        "=r"(v.w[6]), "=r"(v.w[7])
@@ -119,9 +118,7 @@ __device__ __forceinline__ Piece<DT, VEC> load_piece(const void *base, uint64_t 
     return v;
 }
 
-// WIDE: a 32-byte piece (to a 32-byte boundary) in one store, which fills its
-// sector at once.
-template <int DT, int VEC, bool WIDE = false>
+template <int DT, int VEC>
 __device__ __forceinline__ void store_piece(void *base, uint64_t element, const Piece<DT, VEC> &v)
 {
     char *to = static_cast<char *>(base) + element * (DT == M3C_F32 ? 4u : 2u);
@@ -129,7 +126,7 @@ __device__ __forceinline__ void store_piece(void *base, uint64_t element, const 
         *reinterpret_cast<uint16_t *>(to) = static_cast<uint16_t>(v.w[0]);
     } else if constexpr (Piece<DT, VEC>::BYTES == 4) {
         *reinterpret_cast<uint32_t *>(to) = v.w[0];
-    } else if constexpr (Piece<DT, VEC>::BYTES == 32 && (WIDE || VEC == 16)) {
+    } else if constexpr (Piece<DT, VEC>::BYTES == 32) {
         asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v.w[0]), "r"(v.w[1]),
                      "r"(v.w[2]), "r"(v.w[3]), "r"(v.w[4]), "r"(v.w[5]), "r"(v.w[6]), "r"(v.w[7])
                      : "memory");
@@ -168,17 +165,17 @@ __device__ __forceinline__ void widen_piece(const Piece<DT, VEC> &v, float (&x)[
     }
 }
 
-// Eight F32 values as they are stored.
-template <int DT>
-__device__ __forceinline__ Piece<DT, 8> narrow_piece(const float (&x)[8])
+// VEC F32 values as they are stored.
+template <int DT, int VEC>
+__device__ __forceinline__ Piece<DT, VEC> narrow_piece(const float (&x)[VEC])
 {
-    Piece<DT, 8> v;
+    Piece<DT, VEC> v;
     if constexpr (DT == M3C_F32) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v.w[i] = as_bits(x[i]);
+        for (int i = 0; i < VEC; ++i) v.w[i] = as_bits(x[i]);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < VEC / 2; ++i) {
             if constexpr (DT == M3C_BF16) {
                 const __nv_bfloat162 two = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
                 v.w[i] = *reinterpret_cast<const uint32_t *>(&two);
@@ -554,9 +551,14 @@ template <int DT, int MODE>
 int norm_depth(const m3c_norm_e4m3_params &p, bool vectors, bool wide, cudaStream_t stream)
 {
     if constexpr (DT != M3C_F32) {
+        // pieces per thread.  What a thread does once per row (the root, the
+        // divisor) weighs on one piece: many rows of one group take two (16384 x
+        // 4096 bf16 without residual: a tenth less time).  With a divisor per
+        // piece, or too few rows to fill the SMs with a row's fewer threads, one
+        // is faster.  Rows past 8192 elements need four
         const uint64_t pieces = p.width / 16u;
         const bool many = p.rows >= 2048u && MODE == GROUP_ROW;
-        if (wide && pieces > NV16MIN) {
+        if (wide) {
             if (pieces <= 512u && !(many && pieces > 32u)) return norm_launch<DT, MODE, 16, 1>(p, stream);
             if (pieces <= 512u) return norm_launch<DT, MODE, 16, 2>(p, stream);
             return norm_launch<DT, MODE, 16, 4>(p, stream);
@@ -566,13 +568,9 @@ int norm_depth(const m3c_norm_e4m3_params &p, bool vectors, bool wide, cudaStrea
     // 6.4 with eight, which are for the widths that four leave past 1024 threads
     if (!vectors && p.width <= 4096u) return norm_launch<DT, MODE, 1, 4>(p, stream);
     if (!vectors) return norm_launch<DT, MODE, 1, 8>(p, stream);
-    // pieces per thread.  What a thread does once per row (the root, the
-    // divisor) weighs on two pieces: many rows of one group take four (16384 x
-    // 4096 bf16 without residual: a tenth less time).  With a divisor per
-    // piece, or too few rows to fill the SMs with a row's fewer threads, two
-    // are faster (the same rows in groups of 128: 86 us against 90), as with
-    // F32's wider pieces (8192 x 4096 with residual: 70 us against 72).  Rows
-    // past 8192 elements need eight
+    // the same in pieces of eight elements, of which F32's take as many registers
+    // as 16 of the others (8192 x 4096 with residual: 70 us with two, 72 with
+    // four)
     const uint64_t pieces = p.width / 8u;
     const bool many = p.rows >= 2048u && MODE == GROUP_ROW && DT != M3C_F32;
     if (pieces <= 32u) return norm_launch<DT, MODE, 8, 1>(p, stream);
@@ -652,16 +650,16 @@ __device__ __forceinline__ void find_slots(const m3c_cache_params &p, uint32_t f
     }
 }
 
-// The vector kernels: vectors of a multiple of eight elements, rows aligned for
-// 16-byte accesses.  `lanes` lanes (a power of two) own a vector, P pieces of
-// eight elements each, piece j of lane l being number j * lanes + l.  A thread
+// The vector kernels: vectors of whole pieces of VEC elements, rows aligned for
+// them.  `lanes` lanes (a power of two) own a vector, P pieces each, piece j of
+// lane l being number j * lanes + l.  A thread
 // keeps its place (keys or values, head, lane) for several rows; blockIdx.y
 // takes over where a row's vectors do not fit a block.  The slots of a CTA's
 // rows are found once, in shared memory.
 //
 // Bytes bound both directions: three per element of 16-bit rows.  262144 rows
-// of 8 heads of 128 in bf16 are read in 250 us (6.5 TB/s, 0.98 of the measured
-// copy rate), 65536 written in 74.5 us (5.5 TB/s, 0.83), 16384 in 21.1 us (0.73).
+// of 8 heads of 128 in bf16 are read in 249 us (6.5 TB/s, 1.00 of the measured
+// copy rate), 65536 written in 70.7 us (5.8 TB/s, 0.88), 16384 in 20.0 us (0.77).
 // Writing has some twelve instructions an element (the maximum over the vector,
 // a correctly rounded quotient) and the dependent loads that find a slot.
 struct cache_shape {
@@ -703,8 +701,8 @@ struct cache_place {
 
 // Writing: the CTA walks over its rows, the next rows' loads on their way while
 // one row's codes are made; the slots are found behind the first loads.  (One
-// row a CTA, unrolled as reading is: 87 us for the 65536 rows above.)
-template <int DT, int P>
+// row a CTA, unrolled as reading is, took 87 us for the 65536 rows above.)
+template <int DT, int VEC, int P>
 __global__ void __launch_bounds__(CACHE_THREADS, 2)
     cache_write_kernel(const __grid_constant__ m3c_cache_params p, const __grid_constant__ cache_shape shape)
 {
@@ -712,37 +710,37 @@ __global__ void __launch_bounds__(CACHE_THREADS, 2)
     const cache_place at(p, shape);
     const uint64_t token_stride = p.token_stride[at.kv];
     const char *base = static_cast<const char *>(p.rows[at.kv]) +
-                       (at.first * token_stride + at.head * p.head_stride[at.kv] + at.lane * 8u) *
+                       (at.first * token_stride + at.head * p.head_stride[at.kv] + at.lane * VEC) *
                            (DT == M3C_F32 ? 4u : 2u);
-    uint8_t *const codes = p.codes[at.kv] + at.lane * 8u;
+    uint8_t *const codes = p.codes[at.kv] + at.lane * VEC;
     float *const scales = p.scales[at.kv];
     bool inside[P];
 #pragma unroll
-    for (int j = 0; j < P; ++j) inside[j] = at.owner && (j * at.lanes + at.lane) * 8u < p.head_dim;
+    for (int j = 0; j < P; ++j) inside[j] = at.owner && (j * at.lanes + at.lane) * VEC < p.head_dim;
     // the thread's next row, and the way from row to row, in bytes
     const char *row = base + at.side * token_stride * (DT == M3C_F32 ? 4u : 2u);
     const uint64_t stride = shape.rows * token_stride * (DT == M3C_F32 ? 4u : 2u);
-    auto load = [&](uint32_t r, Piece<DT, 8> (&piece)[P]) {
+    auto load = [&](uint32_t r, Piece<DT, VEC> (&piece)[P]) {
 #pragma unroll
         for (int j = 0; j < P; ++j) {
             piece[j] = {};
-            if (inside[j] && r < at.count) piece[j] = load_piece<DT, 8>(row, j * at.lanes * 8u);
+            if (inside[j] && r < at.count) piece[j] = load_piece<DT, VEC>(row, j * at.lanes * VEC);
         }
         row += stride;
     };
-    Piece<DT, 8> next[P];
+    Piece<DT, VEC> next[P];
     load(at.side, next);
     if (threadIdx.x < 32u) find_slots(p, at.first, at.count, slots);
     __syncthreads();
     // the loop's bounds are the block's, so that its shuffles are whole
     for (uint32_t r0 = 0; r0 < at.count; r0 += shape.rows) {
         const uint32_t r = r0 + at.side;
-        float x[P][8];
+        float x[P][VEC];
         float most = 0.0f;
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-            widen_piece<DT, 8>(next[j], x[j]);
-            const float m = largest_of<8>(x[j]);
+            widen_piece<DT, VEC>(next[j], x[j]);
+            const float m = largest_of<VEC>(x[j]);
             asm("max.NaN.f32 %0, %1, %2;" : "=f"(most) : "f"(most), "f"(m));
         }
         load(r + shape.rows, next);
@@ -758,17 +756,17 @@ __global__ void __launch_bounds__(CACHE_THREADS, 2)
             if (at.lane == 0u) scales[vector] = d.scale;
 #pragma unroll
             for (int j = 0; j < P; ++j) {
-                if (inside[j]) e4m3_store<8>(codes + vector * p.head_dim + j * at.lanes * 8u, x[j], d);
+                if (inside[j]) e4m3_store<VEC>(codes + vector * p.head_dim + j * at.lanes * VEC, x[j], d);
             }
         }
     }
 }
 
 // Reading: the slots first, then STEPS rows of a thread at once.  (Walking as
-// writing does: 254 us for the 262144 rows above, 19.9 against 19.0 for 16384.)
-// F32 rows are stored 32 bytes a lane: two stores of 16 filled their sectors in
-// halves, 278 us against 207 for 131072 rows.
-template <int DT, int P, int STEPS>
+// writing does took 254 us for the 262144 rows above.)  Stores of 32 bytes a lane
+// fill their sectors at once: with two of 16 bytes 131072 F32 rows took 278 us,
+// with one 207.
+template <int DT, int VEC, int P, int STEPS>
 __global__ void __launch_bounds__(CACHE_THREADS)
     cache_read_kernel(const __grid_constant__ m3c_cache_params p, const __grid_constant__ cache_shape shape)
 {
@@ -779,10 +777,10 @@ __global__ void __launch_bounds__(CACHE_THREADS)
     if (!at.owner) return;
     const uint64_t token_stride = p.token_stride[at.kv];
     char *const base = static_cast<char *>(p.rows[at.kv]) +
-                       (at.first * token_stride + at.head * p.head_stride[at.kv] + at.lane * 8u) *
+                       (at.first * token_stride + at.head * p.head_stride[at.kv] + at.lane * VEC) *
                            (DT == M3C_F32 ? 4u : 2u);
-    const uint8_t *const from = p.codes[at.kv] + at.lane * 8u;
-    uint2 codes[STEPS][P];
+    const uint8_t *const from = p.codes[at.kv] + at.lane * VEC;
+    e4m3_codes<VEC> codes[STEPS][P];
     float scale[STEPS];
     bool live[STEPS];
 #pragma unroll
@@ -795,8 +793,8 @@ __global__ void __launch_bounds__(CACHE_THREADS)
 #pragma unroll
         for (int j = 0; j < P; ++j) {
             codes[i][j] = {};
-            if (live[i] && (j * at.lanes + at.lane) * 8u < p.head_dim) {
-                codes[i][j] = __ldcs(reinterpret_cast<const uint2 *>(from + vector * p.head_dim + j * at.lanes * 8u));
+            if (live[i] && (j * at.lanes + at.lane) * VEC < p.head_dim) {
+                codes[i][j].load(from + vector * p.head_dim + j * at.lanes * VEC);
             }
         }
     }
@@ -805,11 +803,11 @@ __global__ void __launch_bounds__(CACHE_THREADS)
         const uint32_t r = i * shape.rows + at.side;
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-            float x[8];
-            e4m3_values(codes[i][j], x);
+            float x[VEC];
+            codes[i][j].values(x);
             multiply(x, scale[i]);
-            if (live[i] && (j * at.lanes + at.lane) * 8u < p.head_dim) {
-                store_piece<DT, 8, true>(base, r * token_stride + j * at.lanes * 8u, narrow_piece<DT>(x));
+            if (live[i] && (j * at.lanes + at.lane) * VEC < p.head_dim) {
+                store_piece<DT, VEC>(base, r * token_stride + j * at.lanes * VEC, narrow_piece<DT, VEC>(x));
             }
         }
     }
@@ -857,12 +855,12 @@ __global__ void __launch_bounds__(QUANT_THREADS) cache_any_kernel(const __grid_c
     }
 }
 
-template <int DT, bool WRITE, int P>
+template <int DT, int VEC, bool WRITE, int P>
 int launch_cache_vectors(const m3c_cache_params &p, cudaStream_t stream)
 {
     cache_shape shape;
     shape.lane_shift = 0u;
-    while ((8u * P << shape.lane_shift) < p.head_dim) ++shape.lane_shift;
+    while ((static_cast<uint32_t>(VEC * P) << shape.lane_shift) < p.head_dim) ++shape.lane_shift;
     const uint32_t fit = CACHE_THREADS >> shape.lane_shift;
     const uint32_t all = 2u * p.heads;
     shape.vectors = all < fit ? all : fit;
@@ -878,47 +876,64 @@ int launch_cache_vectors(const m3c_cache_params &p, cudaStream_t stream)
         const uint64_t rounds = (waves - 1u) / CACHE_STEPS + 1u;
         shape.steps = static_cast<uint32_t>((waves - 1u) / rounds + 1u);
         const dim3 grid((p.row_count - 1u) / (shape.rows * shape.steps) + 1u, chunks);
-        cache_write_kernel<DT, P><<<grid, block, 0, stream>>>(p, shape);
+        cache_write_kernel<DT, VEC, P><<<grid, block, 0, stream>>>(p, shape);
     } else {
         // a small batch takes one: the unrolled code's own fetch costs more
         // than it hides
-        constexpr int MANY = P == 1 ? 4 : 2;
+        constexpr int MANY = VEC * P == 8 ? 4 : 2;
         shape.steps = groups < MANY * resident ? 1u : MANY;
         const dim3 grid((p.row_count - 1u) / (shape.rows * shape.steps) + 1u, chunks);
         if (shape.steps == 1u) {
-            cache_read_kernel<DT, P, 1><<<grid, block, 0, stream>>>(p, shape);
+            cache_read_kernel<DT, VEC, P, 1><<<grid, block, 0, stream>>>(p, shape);
         } else {
-            cache_read_kernel<DT, P, MANY><<<grid, block, 0, stream>>>(p, shape);
+            cache_read_kernel<DT, VEC, P, MANY><<<grid, block, 0, stream>>>(p, shape);
         }
     }
     return static_cast<int>(cudaGetLastError());
 }
 
-// The pieces per lane: as few idle lanes as can be (eight elements a piece,
-// lanes a power of two), and of equals the more pieces.
-template <int DT, bool WRITE>
-int launch_cache_pieces(const m3c_cache_params &p, cudaStream_t stream)
+// The pieces per lane of a vector of `dim` elements in pieces of `vec`: as few
+// idle lanes as can be (lanes a power of two, at most a warp), and of equals the
+// more pieces, up to `preferred`.  `idle` becomes the elements that idle lanes
+// would have.
+int cache_pieces(uint32_t dim, uint32_t vec, int most, int preferred, uint32_t *idle)
 {
-    // four pieces of F32, or of rows held while the next are read, leave too few
-    // threads on an SM (65536 rows written: 82 us with four, 76 with two)
-    constexpr int MOST = WRITE || DT == M3C_F32 ? 3 : 4;
-    const uint32_t pieces = p.head_dim / 8u;
+    const uint32_t pieces = dim / vec;
     int best = 1;
-    uint32_t idle = UINT32_MAX;
-    for (int k = 1; k <= MOST; ++k) {
+    *idle = UINT32_MAX;
+    for (int k = 1; k <= most; ++k) {
         uint32_t lanes = 1u;
         while (lanes * k < pieces) lanes <<= 1;
-        if (lanes <= 32u && lanes * k - pieces <= idle) {
-            idle = lanes * k - pieces;
+        const uint32_t rest = (lanes * k - pieces) * vec;
+        if (lanes <= 32u && (rest < *idle || (rest == *idle && k <= preferred))) {
+            *idle = rest;
             best = k;
         }
     }
-    switch (best) {
-    case 1: return launch_cache_vectors<DT, WRITE, 1>(p, stream);
-    case 2: return launch_cache_vectors<DT, WRITE, 2>(p, stream);
-    case 3: return launch_cache_vectors<DT, WRITE, 3>(p, stream);
-    default: return launch_cache_vectors<DT, WRITE, MOST>(p, stream);
+    return best;
+}
+
+// Pieces of 32 bytes (`wide`: the rows are aligned for them) unless pieces of 16
+// leave fewer lanes idle.  More than two pieces of 16 elements to write leave too
+// few threads on an SM; of one and two, one is faster (65536 rows of 8 x 128
+// written in 70.7 against 72.7 us, 262144 read in 249 against 251 us).
+template <int DT, bool WRITE>
+int launch_cache_pieces(const m3c_cache_params &p, bool wide, cudaStream_t stream)
+{
+    uint32_t idle = 0;
+    const int narrow = cache_pieces(p.head_dim, 8u, 3, 3, &idle);
+    if constexpr (DT != M3C_F32) {
+        uint32_t wide_idle = 0;
+        const int k = cache_pieces(p.head_dim, 16u, WRITE ? 2 : 3, 1, &wide_idle);
+        if (wide && wide_idle <= idle) {
+            if (k == 1) return launch_cache_vectors<DT, 16, WRITE, 1>(p, stream);
+            if (k == 2) return launch_cache_vectors<DT, 16, WRITE, 2>(p, stream);
+            return launch_cache_vectors<DT, 16, WRITE, WRITE ? 2 : 3>(p, stream);
+        }
     }
+    if (narrow == 1) return launch_cache_vectors<DT, 8, WRITE, 1>(p, stream);
+    if (narrow == 2) return launch_cache_vectors<DT, 8, WRITE, 2>(p, stream);
+    return launch_cache_vectors<DT, 8, WRITE, 3>(p, stream);
 }
 
 // The first skipped row, and none from here on.
@@ -931,18 +946,23 @@ template <bool WRITE>
 int launch_cache(const m3c_cache_params &p, cudaStream_t stream)
 {
     const uint64_t vectors = static_cast<uint64_t>(p.row_count) * 2u * p.heads;
-    // a vector's lanes are at most a warp of three pieces each; the grid's y
+    // pieces of 32 bytes where the rows are aligned for them, else of 16; a
+    // vector's lanes are at most a warp of three pieces each; the grid's y
     // counts heads
+    const uint32_t size = p.dtype[0] == M3C_F32 ? 4u : 2u;
     bool fits = p.dtype[0] == p.dtype[1] && p.head_dim % 8u == 0u && p.head_dim <= 768u && p.heads <= 16384u;
+    bool wide = p.head_dim % (32u / size) == 0u;
     for (int k = 0; k < 2; ++k) {
-        fits = fits && aligned_to(p.rows[k], p.dtype[0] == M3C_F32 ? 32 : 16) && p.token_stride[k] % 8u == 0u &&
-               p.head_stride[k] % 8u == 0u;
+        const uint64_t address = reinterpret_cast<uintptr_t>(p.rows[k]) | p.token_stride[k] * size |
+                                 p.head_stride[k] * size;
+        fits = fits && address % 16u == 0u;
+        wide = wide && address % 32u == 0u;
     }
-    if (fits) {
+    if (fits && (wide || p.dtype[0] != M3C_F32)) {
         switch (p.dtype[0]) {
-        case M3C_F16: return launch_cache_pieces<M3C_F16, WRITE>(p, stream);
-        case M3C_BF16: return launch_cache_pieces<M3C_BF16, WRITE>(p, stream);
-        default: return launch_cache_pieces<M3C_F32, WRITE>(p, stream);
+        case M3C_F16: return launch_cache_pieces<M3C_F16, WRITE>(p, wide, stream);
+        case M3C_BF16: return launch_cache_pieces<M3C_BF16, WRITE>(p, wide, stream);
+        default: return launch_cache_pieces<M3C_F32, WRITE>(p, wide, stream);
         }
     }
     const unsigned grid = capped_grid((vectors + QUANT_WARPS - 1) / QUANT_WARPS, 32u);
@@ -959,16 +979,17 @@ extern "C" int m3c_launch_norm_e4m3(const m3c_norm_e4m3_params *params, void *st
     m3c_norm_e4m3_params p = *params;
     p.width_reciprocal = 1.0f / static_cast<float>(p.width);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const uint64_t step = p.dtype == M3C_F32 ? 4u : 8u;  // elements of 16 bytes
-    const bool vectors = p.width % 8u == 0u && p.group % 8u == 0u && p.x_stride % step == 0u && aligned_to(p.x, 16) &&
+    // eight elements are one access: 32 bytes of F32, 16 of the others
+    const unsigned bytes = p.dtype == M3C_F32 ? 32u : 16u;
+    const bool vectors = p.width % 8u == 0u && p.group % 8u == 0u && p.x_stride % 8u == 0u && aligned_to(p.x, bytes) &&
                          aligned_to(p.scale, 16) && aligned_to(p.codes, 8) &&
-                         (p.resid_b == nullptr || (p.resid_stride % step == 0u && aligned_to(p.resid_b, 16))) &&
-                         (p.sum_out == nullptr || (p.sum_stride % step == 0u && aligned_to(p.sum_out, 16)));
-    const bool wide = vectors && p.dtype != M3C_F32 && p.width % 16u == 0u && p.group % 16u == 0u &&
+                         (p.resid_b == nullptr || (p.resid_stride % 8u == 0u && aligned_to(p.resid_b, bytes))) &&
+                         (p.sum_out == nullptr || (p.sum_stride % 8u == 0u && aligned_to(p.sum_out, bytes)));
+    // sixteen 16-bit ones 32, where they keep a warp's lanes busy
+    const bool wide = vectors && p.dtype != M3C_F32 && p.width > 256u && p.width % 16u == 0u && p.group % 16u == 0u &&
                       p.x_stride % 16u == 0u && aligned_to(p.x, 32) && aligned_to(p.codes, 16) &&
                       (p.resid_b == nullptr || (p.resid_stride % 16u == 0u && aligned_to(p.resid_b, 32))) &&
-                      (p.sum_out == nullptr || (p.sum_stride % 16u == 0u && aligned_to(p.sum_out, 32))) &&
-                      p.width > 16u * NV16MIN;
+                      (p.sum_out == nullptr || (p.sum_stride % 16u == 0u && aligned_to(p.sum_out, 32)));
     if (p.width <= (vectors ? NORM_WIDEST : NORM_WIDEST / 2u)) {
         switch (p.dtype) {
         case M3C_F16: return norm_mode<M3C_F16>(p, vectors, wide, s);

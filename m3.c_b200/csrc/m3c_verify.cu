@@ -186,7 +186,7 @@ template <int DT, int VEC>
 __global__ void __launch_bounds__(VERIFY_THREADS, 1024 / VERIFY_THREADS)
     verify_kernel(const __grid_constant__ m3c_verify_params p, uint32_t part)
 {
-    constexpr int LOADS = VEC == 1 ? 8 : VEC == 4 ? 4 : 2;  // on their way per lane and model
+    constexpr int LOADS = VEC == 1 ? 8 : VEC == 4 ? 4 : 1;  // on their way per lane and model
     constexpr int PARTS = VERIFY_MOST_CTAS * VERIFY_WARPS;
     __shared__ double mine[2][VERIFY_WARPS];    // the sums of this CTA's parts, per round
     __shared__ double parts[PARTS];
