@@ -117,6 +117,9 @@ def check_norm(h, w, group, codes, scales, epsilon=1e-6):
     (1, 1, 1), (3, 7, 7), (2, 8, 8), (5, 31, 31), (4, 64, 32), (3, 96, 24), (2, 100, 4), (1, 2048, 2048),
     (300, 2048, 128), (33, 2051, 2051), (17, 2051, 7), (9, 4096, 32), (2, 4104, 8), (7, 5120, 160), (3, 8192, 8192),
     (2, 16384, 256), (2, 20000, 20000), (2, 40000, 400), (1, 40001, 40001), (1200, 256, 64), (700, 520, 520),
+    # pieces of 16 and of eight elements, one to eight a thread
+    (40, 528, 528), (40, 528, 16), (40, 528, 48), (3000, 1040, 1040), (2100, 8208, 8208), (5, 16384, 512),
+    (2100, 4104, 4104), (3, 16376, 16376), (2500, 520, 520), (2049, 264, 264),
 ])
 @pytest.mark.parametrize("residual", [False, True])
 def test_norm(m3, gpu, dtype, rows, width, group, residual):
@@ -381,6 +384,10 @@ def laid_out(t, layout):
     elif layout == "heads first":
         wide = torch.full((heads, rows + 3, dim), 5.0, dtype=t.dtype, device="cuda")
         view = wide[:, :rows].transpose(0, 1)
+    elif layout == "sixteen":  # aligned to 16 bytes, not to 32
+        shift = 16 // t.element_size()
+        wide = torch.full((rows * heads * dim + shift,), 5.0, dtype=t.dtype, device="cuda")
+        view = wide[shift:].view(rows, heads, dim)
     elif layout == "odd":      # nothing aligned to a vector
         wide = torch.full((rows * (heads * (dim + 1) + 3) + 1,), 5.0, dtype=t.dtype, device="cuda")
         view = wide[1:].as_strided((rows, heads, dim), (heads * (dim + 1) + 3, dim + 1, 1), 1)
@@ -394,7 +401,9 @@ SHAPES = [
     (1, 1, 1, 1, 5), (2, 3, 8, 3, 40), (7, 5, 80, 48, 90), (3, 8, 128, 16, 70), (33, 2, 64, 16, 9), (70, 1, 128, 64, 4),
     (1, 4, 256, 16, 100), (2, 2, 257, 7, 20), (2, 1, 320, 16, 33), (5, 3, 60, 1, 12), (3, 16, 192, 100, 30),
     (1, 8, 128, 16, 1), (1, 1, 8, 16, 1000), (2, 3, 1032, 4, 9), (300, 2, 16, 8, 3), (3, 2, 576, 16, 30),
-    (2, 1, 768, 16, 20), (2, 1, 776, 16, 20), (1500, 1, 8, 16, 2), (2, 20, 256, 32, 40),
+    (2, 1, 768, 16, 20), (2, 1, 776, 16, 20), (2, 3, 72, 16, 30), (1, 2, 24, 8, 20), (4, 4, 128, 16, 25),
+    (3, 8, 128, 15, 25), (3, 8, 128, 17, 25), (3, 8, 128, 18, 25), (2, 2, 96, 16, 25), (2, 2, 112, 16, 25),
+    (2, 2, 48, 16, 25), (1500, 1, 8, 16, 2), (2, 20, 256, 32, 40),
 ]
 
 
@@ -407,7 +416,8 @@ def test_cache_write_and_read(m3, gpu, dtypes, sequences, heads, dim, page, long
     c = Paged(m3, rng, sequences, heads, dim, page, longest, empty=sequences > 1)
     tokens, slots = c.tokens(), c.slots()
     before = [(a.cpu().numpy().copy(), b.cpu().numpy().copy()) for a, b in zip(c.codes, c.scales)]
-    layouts = [("dense", "fused"), ("heads first", "odd"), ("fused", "fused")][(sequences + dim) % 3]
+    layouts = [("dense", "fused"), ("heads first", "odd"), ("fused", "fused"), ("sixteen", "dense")][
+        (sequences + dim + page) % 4]
     rows = []
     for name, layout in zip(dtypes, layouts):
         v = rng.normal(size=(tokens, heads, dim)) * np.exp(2 * rng.normal(size=(tokens, heads, 1)))
