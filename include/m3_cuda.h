@@ -918,8 +918,9 @@ m3_status m3_cuda_abs_max_static(int device, void *stream, m3_dtype dtype,
  * with every step.  These calls therefore take device addresses and sizes,
  * like m3_cuda_abs_max_static (two of them are graph operators too:
  * M3_OP_RMS_NORM_E4M3 and M3_OP_VERIFY_DRAFT), and are stream-ordered: they check their
- * arguments on the host, enqueue on `stream` (a cudaStream_t of the device;
- * NULL is the legacy default stream) and return without waiting.  They
+ * arguments on the host, enqueue on `stream` (a cudaStream_t of the device
+ * `device`, a CUDA ordinal; NULL is the legacy default stream) and return
+ * without waiting.  They
  * allocate nothing and may be captured into a CUDA graph.  The calling
  * thread's current device is restored before return.  Memory that they name
  * must stay valid until the stream has passed the call; work on other streams
@@ -938,7 +939,9 @@ m3_status m3_cuda_abs_max_static(int device, void *stream, m3_dtype dtype,
 /* RMS norm into E4M3, with the residual's addition:
  *   h = input, or input + residual rounded to `dtype`,
  *   y = h * scale / sqrt(mean(h^2) + epsilon)     (F32; the mean over the row)
- * and each `group` consecutive elements of a row of y quantised together.
+ * and each `group` consecutive elements of a row of y quantised together (the
+ * root is common to a row and leaves the quotients y / scale: they are taken of
+ * h * scale, with two roundings fewer).
  * The row sums run in F32 in a fixed order of their own (not the reference's
  * left-to-right order of M3_OP_RMS_NORM), so results repeat bit for bit; a row
  * whose squares pass the F32 range has y = 0, as its infinite mean says.
