@@ -917,15 +917,15 @@ m3_status m3_cuda_abs_max_static(int device, void *stream, m3_dtype dtype,
  * session is created; the rows, sequences and drafts of a serving step change
  * with every step.  These calls therefore take device addresses and sizes,
  * like m3_cuda_abs_max_static (two of them are graph operators too:
- * M3_OP_RMS_NORM_E4M3 and M3_OP_VERIFY_DRAFT), and are stream-ordered: they check their
- * arguments on the host, enqueue on `stream` (a cudaStream_t of the device
- * `device`, a CUDA ordinal; NULL is the legacy default stream) and return
- * without waiting.  They
- * allocate nothing and may be captured into a CUDA graph.  The calling
- * thread's current device is restored before return.  Memory that they name
- * must stay valid until the stream has passed the call; work on other streams
- * is ordered by the caller's events.  A refused call enqueues nothing and
- * writes nothing.
+ * M3_OP_RMS_NORM_E4M3 and M3_OP_VERIFY_DRAFT), and are stream-ordered: they
+ * check their arguments on the host, enqueue on `stream` (a cudaStream_t of
+ * the device `device`, a CUDA ordinal, or of the cache's; NULL is the legacy
+ * default stream) and return without waiting.  They allocate nothing and may
+ * be captured into a CUDA graph.  The calling thread's current device is
+ * restored before return.  Memory that they name must stay valid, and inputs
+ * unchanged, until the stream has passed the call; work on other streams is
+ * ordered by the caller's events.  A refused call enqueues nothing and writes
+ * nothing.
  *
  * 8-bit values are E4M3 (one sign, four exponent and three significand bits,
  * largest value 448, no infinity), quantised in groups that share one F32

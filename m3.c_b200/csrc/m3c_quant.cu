@@ -317,6 +317,7 @@ __global__ void __launch_bounds__(norm_block(VEC, K))
     __shared__ float part[32];
     __shared__ uint32_t top[32];
     if (p.status != nullptr) {
+        // no launch that can fail runs beside this one: the same for all threads
         if (failed_before(p.status, p.skip_before)) return;
         if (p.first_of_run && blockIdx.x == 0 && threadIdx.x == 0 && threadIdx.y == 0) {
             atomicAdd(&p.status->runs_started, 1u);
@@ -463,6 +464,7 @@ __global__ void __launch_bounds__(QUANT_THREADS)
     const int warp = static_cast<int>(threadIdx.x) / 32;
     const int lane = static_cast<int>(threadIdx.x) % 32;
     if (p.status != nullptr) {
+        // no launch that can fail runs beside this one: the same for all threads
         if (failed_before(p.status, p.skip_before)) return;
         if (p.first_of_run && blockIdx.x == 0 && threadIdx.x == 0) atomicAdd(&p.status->runs_started, 1u);
     }

@@ -199,6 +199,9 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 1024 / VERIFY_THREADS)
     __shared__ uint32_t found;
     __shared__ uint32_t last_positive;
     if (p.status != nullptr) {
+        // the same for all threads of a cluster: a session runs launches side by
+        // side only where none of them can fail, so the status does not change
+        // meanwhile
         if (failed_before(p.status, p.skip_before)) return;
         if (p.first_of_run && blockIdx.x == 0 && threadIdx.x == 0) atomicAdd(&p.status->runs_started, 1u);
     }
