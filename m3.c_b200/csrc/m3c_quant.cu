@@ -1001,9 +1001,12 @@ extern "C" int m3c_launch_norm_e4m3(const m3c_norm_e4m3_params *params, void *st
     }
     const size_t row_bytes = p.width * sizeof(float);
     const bool kept = row_bytes <= NORM_KEPT_BYTES;
-    if (kept && row_bytes > 48u * 1024u) {
-        cudaFuncSetAttribute(norm_e4m3_any_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(NORM_KEPT_BYTES));
+    if (kept) {
+        // these rows begin at 32 KB; with the kernel's static shared memory they pass
+        // the default of 48 KB below 12288 elements
+        const cudaError_t code = cudaFuncSetAttribute(
+            norm_e4m3_any_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(NORM_KEPT_BYTES));
+        if (code != cudaSuccess) return static_cast<int>(code);
     }
     norm_e4m3_any_kernel<<<capped_grid(p.rows, 32u), QUANT_THREADS, kept ? row_bytes : 0u, s>>>(p, kept ? 1 : 0);
     return static_cast<int>(cudaGetLastError());
