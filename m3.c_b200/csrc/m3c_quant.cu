@@ -602,8 +602,9 @@ __device__ __forceinline__ int64_t slot_in_sequence(const m3c_cache_params &p, u
     if (row < begin || row >= p.offsets[s + 1]) return -1;
     const int64_t position = (p.starts != nullptr ? static_cast<int64_t>(p.starts[s]) : 0) + row - begin;
     uint32_t reason = M3C_CACHE_BAD_POSITION;
-    // positions below 2^32 fit the 32-bit division
-    if (position >= 0) {
+    // positions below 2^32 fit the 32-bit division; a negative first offset can give
+    // greater ones
+    if (position >= 0 && position <= UINT32_MAX) {
         const uint32_t at = static_cast<uint32_t>(position) / p.page_tokens;
         if (at < p.page_table_stride) {
             const int64_t page = p.page_table[s * p.page_table_stride + at];
