@@ -21,6 +21,7 @@ namespace m3c {
 constexpr float E4M3_LARGEST = 448.0f;
 constexpr float E4M3_LARGEST_RECIPROCAL = 1.0f / 448.0f;
 constexpr float E4M3_SMALLEST_SCALE = 0x1p-126f;
+constexpr float E4M3_CERTAIN_SCALE = 0x1p119f;  // 448 times any below it is finite
 // div_markstein's remainder v - q s is a multiple of ulp(q) ulp(s).  Quotients
 // below 2^-10 have the code 0 however they round, and for the others the
 // remainder is exact while 2^-33 * 2^-23 s >= 2^-149.

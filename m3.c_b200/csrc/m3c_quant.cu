@@ -284,8 +284,8 @@ __device__ __forceinline__ void multiply(float (&a)[N], float b)
 // The divisor of a group whose largest |z| is `most`.  A code is that of y / s =
 // (z inverse) / s, and as s is the group's largest |y| / 448, that of z over the
 // largest |z| / 448: the inverse root drops out, and with it two roundings.
-// Where a scale is at its lower bound, or not finite, the quotient is taken of y
-// itself (`normed`).
+// Where a scale is at its lower bound, not finite, or so large that the group's y
+// may pass the F32 range, the quotient is taken of y itself (`normed`).
 struct norm_divisor {
     e4m3_divisor by;
     float scale;
@@ -297,7 +297,8 @@ __device__ __forceinline__ norm_divisor divide_norm_by(float most, float inverse
     norm_divisor d;
     const float of_z = e4m3_scale(magnitude_bits(most));
     d.scale = __fmul_rn(of_z, inverse);
-    d.normed = !(of_z > E4M3_SMALLEST_SCALE && d.scale > E4M3_SMALLEST_SCALE);  // a NaN too
+    d.normed = !(of_z > E4M3_SMALLEST_SCALE && d.scale > E4M3_SMALLEST_SCALE &&
+                 d.scale < E4M3_CERTAIN_SCALE);  // a NaN too
     if (d.normed) d.scale = e4m3_scale(magnitude_bits(__fmul_rn(most, inverse)));
     d.by = e4m3_divide_by(d.normed ? d.scale : of_z);
     return d;

@@ -14,7 +14,8 @@ import sys
 import numpy as np
 import pytest
 
-from test_gpu_serving import cache_rows, device_view
+from test_gpu_serving import (TINY, U, cache_rows, device_view, e4m3_table, host, nearest_e4m3, run_norm,
+                              torch_dtype)
 
 pytestmark = pytest.mark.gpu
 
@@ -76,3 +77,57 @@ def test_cache_positions_past_32_bits(m3, gpu, heads, dim):
     c.synchronize()
     written = device_view(c.pointers()[1], (8 * page, heads), "<f4").any(-1).cpu().numpy()
     assert np.array_equal(np.nonzero(written)[0], np.arange(20, 50))
+
+
+def check_norm_ranges(h, w, group, codes, scales, epsilon):
+    """test_gpu_serving.check_norm, with the groups that hold a y past the F32 range (or of an infinite h) NaN, and
+    y = 0 in the rows whose squares pass it."""
+    rows, width = h.shape
+    slack = ((width / 32 + 32) / 2 + 8) * U
+    h, w, epsilon = host(h), host(w), float(np.float32(epsilon))
+    with np.errstate(invalid="ignore", over="ignore"):
+        squares = np.sum(h * h, -1, keepdims=True)
+        inverse = np.where(squares < 2.0 ** 128, 1 / np.sqrt(squares / width + epsilon), 0.0)
+        y = (h * inverse * w).reshape(rows, -1, group)
+    bad = ~(np.abs(y) < 2.0 ** 128 * (1 - 2.0 ** -25)).all(-1)
+    got_scale, got = host(scales), e4m3_table()[codes.cpu().numpy()].reshape(y.shape)
+    assert np.all(np.isnan(got_scale[bad])) and np.all(np.isnan(got[bad]))
+    y, got, got_scale = y[~bad], got[~bad], got_scale[~bad]
+    scale = np.maximum(np.abs(y).max(-1) / 448.0, TINY)
+    assert np.all(np.abs(got_scale - scale) <= slack * scale)
+    q = y / scale[..., None]
+    low, high = np.minimum(q * (1 - 2 * slack), q * (1 + 2 * slack)), np.maximum(q * (1 - 2 * slack), q * (1 + 2 * slack))
+    assert np.all((nearest_e4m3(low) <= got) & (got <= nearest_e4m3(high)))
+    return bad
+
+
+# the register kernel by rows, lanes and words, in vectors and single elements, and the kernel for any width
+FORMS = [(512, 512), (512, 64), (528, 48), (515, 515), (515, 5), (515, 103), (20001, 20001), (20001, 59)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("width, group", FORMS)
+def test_norm_y_past_the_range(m3, gpu, dtype, width, group):
+    """Large weights: a y past the F32 range makes its group NaN, one at its end does not, while h * w stays small."""
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(width + group)
+    x = (0.01 * torch.randn(5, width, generator=g, device="cuda")).to(torch_dtype(dtype))
+    w = torch.ones(width, device="cuda")
+    w[2 * group - 1 if 2 * group < width else width - 1] = 1e38
+    x[:, 2 * group - 1 if 2 * group < width else width - 1] = torch.tensor([0.001, 0.02, 0.06, -0.08, 0.0])
+    bad = check_norm_ranges(x, w, group, *run_norm(m3, x, w, group), 1e-6)
+    assert bad.sum() == 2 and bad[2:4].any(-1).all()
+
+
+def test_norm_scale_past_the_range(m3, gpu):
+    """One element that carries its row: y / 448 itself is past the F32 range."""
+    import torch
+
+    width = 600000
+    x = torch.zeros(2, width, device="cuda")
+    x[0, 77] = 0.01
+    x[1] = 0.01
+    w = torch.full((width,), 3e38, device="cuda")
+    bad = check_norm_ranges(x, w, width, *run_norm(m3, x, w, width, epsilon=1e-12), 1e-12)
+    assert bad.tolist() == [[True], [False]]
