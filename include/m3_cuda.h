@@ -938,13 +938,15 @@ m3_status m3_cuda_abs_max_static(int device, void *stream, m3_dtype dtype,
 
 /* RMS norm into E4M3, with the residual's addition:
  *   h = input, or input + residual rounded to `dtype`,
- *   y = h * scale / sqrt(mean(h^2) + epsilon)     (F32; the mean over the row)
+ *   y = h / sqrt(mean(h^2) + epsilon) * scale     (F32; the mean over the row)
  * and each `group` consecutive elements of a row of y quantised together (the
  * root is common to a row and leaves the quotients y / scale: they are taken of
- * h * scale, with two roundings fewer).
+ * h * scale, with two roundings fewer, but in groups where that product leaves
+ * the F32 range or comes near its lower end).
  * The row sums run in F32 in a fixed order of their own (not the reference's
  * left-to-right order of M3_OP_RMS_NORM), so results repeat bit for bit; a row
- * whose squares pass the F32 range has y = 0, as its infinite mean says.
+ * whose squares pass the F32 range has y = 0 wherever h and scale are finite, as
+ * its infinite mean says.
  * `sum` (may be NULL) receives h.  It may be the very tensor `input` or
  * `residual` (same address and row stride); no other output may overlap an
  * input or another output (M3_STATUS_INVALID_ARGUMENT; the byte spans are

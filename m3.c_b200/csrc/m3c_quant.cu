@@ -285,23 +285,106 @@ __device__ __forceinline__ void multiply(float (&a)[N], float b)
 // (z inverse) / s, and as s is the group's largest |y| / 448, that of z over the
 // largest |z| / 448: the inverse root drops out, and with it two roundings.
 // Where a scale is at its lower bound, not finite, or so large that the group's y
-// may pass the F32 range, the quotient is taken of y itself (`normed`).
+// may pass the F32 range, the quotient is taken of y itself (`normed`).  Where a z
+// passed the range, or the largest is so small that others have lost bits below
+// it, y is made `anew` from h.
 struct norm_divisor {
     e4m3_divisor by;
     float scale;
     bool normed;
+    bool anew;
 };
+
+// A z below 2^-126 is off by 2^-150 at most: nothing against the smallest code of
+// a group whose largest z is not below 2^-102.  Where all are 0, the y of none is
+// above 2^-150 times the inverse root, and all codes 0 while that root is below
+// 2^13 (rows of zeros under an ordinary epsilon).
+constexpr float NORM_LEAST_Z = 0x1p-102f;
+constexpr float NORM_LEAST_SCALE = 0x1p-110f;  // of a group whose largest z is above it
+constexpr float NORM_ZERO_INVERSE = 0x1p13f;
+
+// Whether a group whose largest |z| is `most` is made anew.
+__device__ __forceinline__ bool norm_left_range(float most, float inverse)
+{
+    // a NaN among the z, or in the row (its inverse root), is one of the group's y too
+    return inverse == inverse && (magnitude_bits(most) == 0x7f800000u ||
+                                  (most < NORM_LEAST_Z && !(most == 0.0f && inverse < NORM_ZERO_INVERSE)));
+}
 
 __device__ __forceinline__ norm_divisor divide_norm_by(float most, float inverse)
 {
     norm_divisor d;
     const float of_z = e4m3_scale(magnitude_bits(most));
     d.scale = __fmul_rn(of_z, inverse);
-    d.normed = !(of_z > E4M3_SMALLEST_SCALE && d.scale > E4M3_SMALLEST_SCALE &&
+    d.normed = !(of_z > NORM_LEAST_SCALE && d.scale > E4M3_SMALLEST_SCALE &&
                  d.scale < E4M3_CERTAIN_SCALE);  // a NaN too
-    if (d.normed) d.scale = e4m3_scale(magnitude_bits(__fmul_rn(most, inverse)));
+    d.anew = false;
+    if (d.normed) {
+        d.anew = norm_left_range(most, inverse);
+        d.scale = e4m3_scale(magnitude_bits(__fmul_rn(most, inverse)));
+    }
     d.by = e4m3_divide_by(d.normed ? d.scale : of_z);
     return d;
+}
+
+// h as it was normed: the stored sum (which may lie in the input's memory by now),
+// or the input.
+__device__ __forceinline__ float norm_input(const m3c_norm_e4m3_params &p, uint64_t row, uint64_t j)
+{
+    if (p.sum_out != nullptr) return load_element(p.sum_out, p.dtype, row * p.sum_stride + j);
+    const float x = load_element(p.x, p.dtype, row * p.x_stride + j);
+    if (p.resid_b == nullptr) return x;
+    return round_to(p.dtype, __fadd_rn(x, load_element(p.resid_b, p.dtype, row * p.resid_stride + j)));
+}
+
+// y from h: the root first, which brings h near 1 wherever its square was in range.
+__device__ __forceinline__ float norm_anew(const m3c_norm_e4m3_params &p, float h, uint64_t j, float inverse)
+{
+    return __fmul_rn(__fmul_rn(h, inverse), load_element(p.scale, p.scale_dtype, j));
+}
+
+// A thread's codes of the register kernel once more, pieces of `run` elements: those
+// of the groups that left the range, made anew from h.  Rare, so nothing is kept for
+// it from the pass before, and each thread reads its groups for itself (the warps
+// of a row that is one group share the reading).  The row's h, if it was stored, is
+// visible to it: a barrier of the row's warps is behind the stores.
+template <bool ROW>
+__device__ __noinline__ void norm_anew_codes(const m3c_norm_e4m3_params &p, float inverse, uint32_t run)
+{
+    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+    const uint32_t width = static_cast<uint32_t>(p.width);
+    const uint32_t group = static_cast<uint32_t>(p.group);
+    uint32_t known = width;  // the group whose divisor is known
+    e4m3_divisor d = {};
+    bool wanted = false;
+#pragma unroll 1
+    for (uint32_t at = threadIdx.x * run; ROW || at < width; at += blockDim.x * run) {
+        const uint32_t g = ROW ? 0u : at / group;
+        if (g != known) {
+            known = g;
+            uint32_t most_z = 0u;
+            uint32_t most_y = 0u;
+#pragma unroll 1
+            for (uint32_t j = ROW ? threadIdx.x % 32u : 0u; j < group; j += ROW ? 32u : 1u) {
+                const float h = norm_input(p, row, g * group + j);
+                const uint32_t z = magnitude_bits(__fmul_rn(h, load_element(p.scale, p.scale_dtype, g * group + j)));
+                const uint32_t y = magnitude_bits(norm_anew(p, h, g * group + j, inverse));
+                most_z = z > most_z ? z : most_z;
+                most_y = y > most_y ? y : most_y;
+            }
+            if (ROW) most_y = warp_max(most_y);
+            wanted = ROW || norm_left_range(as_float(most_z), inverse);
+            d = e4m3_divide_by(e4m3_scale(most_y));
+        }
+        if (at >= width) break;
+        if (!wanted) continue;
+        if (at == g * group) p.code_scales[row * (width / group) + g] = d.scale;
+#pragma unroll 1
+        for (uint32_t j = at; j < at + run; ++j) {
+            const float y[1] = {norm_anew(p, norm_input(p, row, j), j, inverse)};
+            e4m3_store<1>(static_cast<uint8_t *>(p.codes) + row * width + j, y, d);
+        }
+    }
 }
 
 // The most threads of a CTA of the register kernel, as norm_depth chooses K.
@@ -435,8 +518,14 @@ __global__ void __launch_bounds__(norm_block(VEC, K))
     norm_divisor d;
     if constexpr (MODE == GROUP_ROW) {
         d = divide_norm_by(as_float(largest), inverse);
+        if (d.anew) {  // the same for the row's threads
+            __syncwarp();
+            norm_anew_codes<true>(p, inverse, VEC);
+            return;
+        }
         if (tid == 0) p.code_scales[row] = d.scale;
     }
+    bool anew = false;
     uint8_t *codes = static_cast<uint8_t *>(p.codes) + row * width;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -446,10 +535,15 @@ __global__ void __launch_bounds__(norm_block(VEC, K))
             const uint32_t g = group_of(at);
             if constexpr (MODE == GROUP_WORDS) most[k] = as_float(words[place + g]);
             d = divide_norm_by(most[k], inverse);
+            anew = anew || d.anew;
             if (at == g * group) p.code_scales[row * groups + g] = d.scale;
         }
         if (d.normed) multiply(z[k], inverse);
         e4m3_store<VEC>(codes + at, z[k], d.by);
+    }
+    if constexpr (MODE != GROUP_ROW) {
+        __syncwarp();
+        if (anew) norm_anew_codes<false>(p, inverse, VEC);
     }
 }
 
@@ -471,18 +565,13 @@ __global__ void __launch_bounds__(QUANT_THREADS)
     }
     const uint64_t groups = p.width / p.group;
     for (uint64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        const uint64_t x0 = row * p.x_stride;
-        const uint64_t r0 = row * p.resid_stride;
-        const uint64_t s0 = row * p.sum_stride;
-        auto read = [&](uint64_t j) {
-            float h = load_element(p.x, p.dtype, x0 + j);
-            if (p.resid_b != nullptr) h = round_to(p.dtype, __fadd_rn(h, load_element(p.resid_b, p.dtype, r0 + j)));
-            return h;
-        };
         float squares = 0.0f;
         for (uint64_t j = threadIdx.x; j < p.width; j += QUANT_THREADS) {
-            const float h = read(j);
-            if (p.sum_out != nullptr) store_element(p.sum_out, p.dtype, s0 + j, h);
+            float h = load_element(p.x, p.dtype, row * p.x_stride + j);
+            if (p.resid_b != nullptr) {
+                h = round_to(p.dtype, __fadd_rn(h, load_element(p.resid_b, p.dtype, row * p.resid_stride + j)));
+            }
+            if (p.sum_out != nullptr) store_element(p.sum_out, p.dtype, row * p.sum_stride + j, h);
             if (kept) held[j] = h;
             squares = __fmaf_rn(h, h, squares);
         }
@@ -493,12 +582,9 @@ __global__ void __launch_bounds__(QUANT_THREADS)
         for (int w = 0; w < QUANT_WARPS; ++w) squares = __fadd_rn(squares, part[w]);
         const float inverse =
             __frsqrt_rn(__fadd_rn(__fmul_rn(squares, p.width_reciprocal), p.epsilon));
+        auto input = [&](uint64_t j) { return kept ? held[j] : norm_input(p, row, j); };
         auto weighted = [&](uint64_t j) {
-            // the stored sum is h (and may be the input's own storage by now)
-            const float h = kept                   ? held[j]
-                            : p.sum_out != nullptr ? load_element(p.sum_out, p.dtype, s0 + j)
-                                                   : read(j);
-            return __fmul_rn(h, load_element(p.scale, p.scale_dtype, j));
+            return __fmul_rn(input(j), load_element(p.scale, p.scale_dtype, j));
         };
         uint8_t *codes = static_cast<uint8_t *>(p.codes) + row * p.width;
         // many groups: one warp each; few: the whole CTA one after another
@@ -507,23 +593,44 @@ __global__ void __launch_bounds__(QUANT_THREADS)
         const uint32_t from = alone ? lane : threadIdx.x;
         for (uint64_t g = alone ? warp : 0; g < groups; g += alone ? QUANT_WARPS : 1) {
             const uint64_t g0 = g * p.group;
+            // of what the threads that share a group found
+            auto join = [&](uint32_t m) {
+                m = warp_max(m);
+                if (!alone) {
+                    if (lane == 0) top[warp] = m;
+                    __syncthreads();
+                    for (int w = 0; w < QUANT_WARPS; ++w) m = top[w] > m ? top[w] : m;
+                }
+                return m;
+            };
             uint32_t largest = 0u;
             for (uint64_t j = from; j < p.group; j += step) {
                 const uint32_t m = magnitude_bits(weighted(g0 + j));
                 largest = m > largest ? m : largest;
             }
-            largest = warp_max(largest);
-            if (!alone) {
-                if (lane == 0) top[warp] = largest;
-                __syncthreads();
-                for (int w = 0; w < QUANT_WARPS; ++w) largest = top[w] > largest ? top[w] : largest;
-            }
-            const norm_divisor d = divide_norm_by(as_float(largest), inverse);
-            if (from == 0) p.code_scales[row * groups + g] = d.scale;
-            for (uint64_t j = from; j < p.group; j += step) {
-                float z[1] = {weighted(g0 + j)};
-                if (d.normed) multiply(z, inverse);
-                e4m3_store<1>(codes + g0 + j, z, d.by);
+            const norm_divisor d = divide_norm_by(as_float(join(largest)), inverse);
+            if (!d.anew) {
+                if (from == 0) p.code_scales[row * groups + g] = d.scale;
+                for (uint64_t j = from; j < p.group; j += step) {
+                    float z[1] = {weighted(g0 + j)};
+                    if (d.normed) multiply(z, inverse);
+                    e4m3_store<1>(codes + g0 + j, z, d.by);
+                }
+            } else {  // rare, and the same for all threads that share the group
+                if (!alone) __syncthreads();
+                largest = 0u;
+#pragma unroll 1
+                for (uint64_t j = from; j < p.group; j += step) {
+                    const uint32_t m = magnitude_bits(norm_anew(p, input(g0 + j), g0 + j, inverse));
+                    largest = m > largest ? m : largest;
+                }
+                const e4m3_divisor by = e4m3_divide_by(e4m3_scale(join(largest)));
+                if (from == 0) p.code_scales[row * groups + g] = by.scale;
+#pragma unroll 1
+                for (uint64_t j = from; j < p.group; j += step) {
+                    const float y[1] = {norm_anew(p, input(g0 + j), g0 + j, inverse)};
+                    e4m3_store<1>(codes + g0 + j, y, by);
+                }
             }
             if (!alone) __syncthreads();
         }

@@ -131,3 +131,61 @@ def test_norm_scale_past_the_range(m3, gpu):
     w = torch.full((width,), 3e38, device="cuda")
     bad = check_norm_ranges(x, w, width, *run_norm(m3, x, w, width, epsilon=1e-12), 1e-12)
     assert bad.tolist() == [[True], [False]]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("width, group", FORMS)
+def test_norm_squares_past_the_range(m3, gpu, dtype, width, group):
+    """y = 0 in a row whose squares pass the F32 range, whatever its weights."""
+    import torch
+
+    x = torch.randn(4, width, device="cuda", generator=torch.Generator(device="cuda").manual_seed(width))
+    x[0] = 2e38
+    x[1, 3] = -3e38
+    x = x.to(torch_dtype(dtype))
+    x[3, 0] = float("inf")
+    w = torch.full((width,), 4.0, device="cuda")
+    codes, scales = run_norm(m3, x, w, group)
+    bad = check_norm_ranges(x, w, group, codes, scales, 1e-6)
+    assert bad.sum() == 1 and bad[3, 0]
+    assert not bool((codes[:2] & 0x7f).any()) and np.all(host(scales[:2]) == TINY)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("width, group", FORMS)
+@pytest.mark.parametrize("h, weight, epsilon", [(1e16, 1e25, 1e-6), (1e-30, 1e-12, 1e-30), (1e-25, 1e-22, 1e-36)])
+@pytest.mark.parametrize("residual", [None, "sum", "in place", "no sum"])
+def test_norm_products_past_the_range(m3, gpu, dtype, width, group, h, weight, epsilon, residual):
+    """h * w leaves the F32 range at either end, y does not; in some groups of some rows."""
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(width + group)
+    t = torch_dtype(dtype)
+    x = torch.randn(6, width, generator=g, device="cuda")
+    x[::2] *= h
+    x = x.to(t)
+    w = torch.randn(width, generator=g, device="cuda")
+    w[width // 3:] *= weight
+    r = total = None
+    stored = x
+    if residual:
+        r = (0.5 * x.float().roll(1, 1)).to(t)
+        stored = (x.float() + r.float()).to(t)
+        total = {"sum": torch.zeros_like(x), "in place": x.clone(), "no sum": None}[residual]
+    given = total if residual == "in place" else x
+    codes, scales = run_norm(m3, given, w, group, r, total, epsilon=epsilon)
+    assert not check_norm_ranges(stored, w, group, codes, scales, epsilon).any()
+    if total is not None:
+        assert torch.equal(total, stored)
+
+
+def test_norm_zero_rows_with_a_small_epsilon(m3, gpu):
+    import torch
+
+    for width, group in FORMS:
+        x = torch.zeros(3, width, device="cuda")
+        x[1] = 1.0
+        w = torch.ones(width, device="cuda")
+        codes, scales = run_norm(m3, x, w, group, epsilon=1e-20)
+        check_norm_ranges(x, w, group, codes, scales, 1e-20)
+        assert not bool((codes[::2] & 0x7f).any()) and np.all(host(scales[::2]) == TINY)
