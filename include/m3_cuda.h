@@ -944,7 +944,8 @@ m3_status m3_cuda_abs_max_static(int device, void *stream, m3_dtype dtype,
  * h * scale, with two roundings fewer, but in groups where that product leaves
  * the F32 range or comes near its lower end).
  * The row sums run in F32 in a fixed order of their own (not the reference's
- * left-to-right order of M3_OP_RMS_NORM), so results repeat bit for bit; a row
+ * left-to-right order of M3_OP_RMS_NORM; no chain of F32 additions is longer than
+ * 300), so results repeat bit for bit; a row
  * whose squares pass the F32 range has y = 0 wherever h and scale are finite, as
  * its infinite mean says.
  * `sum` (may be NULL) receives h.  It may be the very tensor `input` or

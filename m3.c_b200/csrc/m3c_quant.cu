@@ -19,6 +19,7 @@ constexpr int QUANT_WARPS = QUANT_THREADS / 32;
 constexpr int NORM_THREADS = 128;                   // rows share a CTA up to these
 constexpr uint64_t NORM_WIDEST = 16384;             // of the register kernel
 constexpr uint64_t NORM_KEPT_BYTES = 200u * 1024u;  // of shared memory for a row
+constexpr uint32_t NORM_CHAIN = 256;                // squares summed one by one
 
 __device__ __forceinline__ float warp_sum(float v)
 {
@@ -565,7 +566,11 @@ __global__ void __launch_bounds__(QUANT_THREADS)
     }
     const uint64_t groups = p.width / p.group;
     for (uint64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        // chains of at most NORM_CHAIN squares, whose sums join in 64 bits: a longer chain
+        // of like squares drifts by its length in roundings
         float squares = 0.0f;
+        double before = 0.0;
+        uint32_t chain = 0;
         for (uint64_t j = threadIdx.x; j < p.width; j += QUANT_THREADS) {
             float h = load_element(p.x, p.dtype, row * p.x_stride + j);
             if (p.resid_b != nullptr) {
@@ -573,8 +578,15 @@ __global__ void __launch_bounds__(QUANT_THREADS)
             }
             if (p.sum_out != nullptr) store_element(p.sum_out, p.dtype, row * p.sum_stride + j, h);
             if (kept) held[j] = h;
+            if (chain == NORM_CHAIN) {
+                before += static_cast<double>(squares);
+                squares = 0.0f;
+                chain = 0;
+            }
+            ++chain;
             squares = __fmaf_rn(h, h, squares);
         }
+        squares = static_cast<float>(before + static_cast<double>(squares));
         squares = warp_sum(squares);
         if (lane == 0) part[warp] = squares;
         __syncthreads();

@@ -189,3 +189,22 @@ def test_norm_zero_rows_with_a_small_epsilon(m3, gpu):
         codes, scales = run_norm(m3, x, w, group, epsilon=1e-20)
         check_norm_ranges(x, w, group, codes, scales, 1e-20)
         assert not bool((codes[::2] & 0x7f).any()) and np.all(host(scales[::2]) == TINY)
+
+
+def test_norm_millions_of_elements_a_row(m3, gpu):
+    """A row's squares are summed in chains of at most 256, whose sums join in 64 bits: chains and lanes are off by
+    (256 + 32) / 2 steps at most, the root takes half of that, the rest is 8 steps as elsewhere."""
+    import torch
+
+    width = 4194305
+    x = torch.full((1, width), 0.7, device="cuda")
+    x[0, 5] = 3.0
+    w = torch.ones(width, device="cuda")
+    codes, scales = run_norm(m3, x, w, width)
+    h = host(x)
+    y = h / np.sqrt(np.mean(h * h) + 1e-6)
+    slack = ((256 + 32) / 2 + 8) * U
+    scale = np.abs(y).max() / 448
+    assert abs(host(scales)[0, 0] - scale) <= slack * scale
+    got = e4m3_table()[codes.cpu().numpy()]
+    assert np.array_equal(got, nearest_e4m3(y / scale))
