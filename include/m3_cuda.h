@@ -625,6 +625,16 @@ m3_status m3_cuda_graph_plan(const m3_graph *graph,
                              m3_cuda_plan_report *report, char *text,
                              size_t text_capacity, m3_error *error);
 
+/* Which launches of that plan run at the same time: waves[i] becomes the number
+ * of launch i's wave, for the first `capacity` launches (in the order of the
+ * plan's description), *launch_count (may be NULL) how many there are.  The
+ * launches of a wave share no memory and none of the plan can fail; waves run
+ * one after another.  Needs no GPU. */
+m3_status m3_cuda_graph_waves(const m3_graph *graph,
+                              const m3_cuda_session_options *cuda,
+                              uint32_t *waves, size_t capacity,
+                              size_t *launch_count, m3_error *error);
+
 /* ------------------------------------------------------------------------
  * Sharding: one fixed graph split across the GPUs of a box
  * ------------------------------------------------------------------------

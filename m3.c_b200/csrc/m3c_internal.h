@@ -169,7 +169,13 @@ typedef struct {
     size_t *flip_slot;
     uint32_t *flip_command;
     size_t flip_count;
+    /* the wave of each launch: those of one wave may run at the same time */
+    uint32_t *launch_wave;
 } m3c_plan;
+
+/* Launches of one run that may execute at the same time: up to
+ * 1 + M3C_SIDE_STREAMS per wave. */
+#define M3C_SIDE_STREAMS 3
 
 m3_status m3c_plan_build(const m3_graph *graph, bool fuse, m3c_plan *plan,
                          m3_error *error);

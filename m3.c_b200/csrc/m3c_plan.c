@@ -1173,6 +1173,7 @@ static m3_status plan_categorical(planner *p, size_t n, m3_error *error)
     launch.row_sum_out.value = NO_VALUE;
     launch.row_out2.value = NO_VALUE;
     launch.row_out3.value = NO_VALUE;
+    launch.row_out4.value = NO_VALUE;
     launch.norm_scale.value = NO_VALUE;
     launch.norm_bias.value = NO_VALUE;
     launch.command_a = (uint32_t)n;
@@ -1236,6 +1237,7 @@ static m3_status plan_norm(planner *p, size_t n, size_t residual,
     launch.row_sum_out.value = NO_VALUE;
     launch.row_out2.value = NO_VALUE;
     launch.row_out3.value = NO_VALUE;
+    launch.row_out4.value = NO_VALUE;
     launch.command_a = (uint32_t)n;
     launch.command_b = UINT32_MAX;
     if (residual != SIZE_MAX) {
@@ -1445,6 +1447,7 @@ void m3c_plan_free(m3c_plan *plan)
     free(plan->launches);
     free(plan->flip_slot);
     free(plan->flip_command);
+    free(plan->launch_wave);
     memset(plan, 0, sizeof(*plan));
 }
 
@@ -1525,6 +1528,90 @@ static m3_status mark_needed_slots(const m3_graph *graph, m3c_plan *plan,
     return M3_STATUS_OK;
 }
 
+/* Slots a launch reads or writes (both buffers of a slot count as one). */
+static size_t launch_slots(const m3c_plan *plan, const m3c_launch *l,
+                           size_t *slots, size_t capacity)
+{
+    m3c_ref refs[M3C_EW_MAX_OPERANDS + M3C_EW_MAX_OUTPUTS + 12];
+    size_t n = 0U;
+    size_t count = 0U;
+    size_t i;
+    int k;
+
+    if (l->kind == M3C_LAUNCH_EW) {
+        for (k = 0; k < l->n_operands; ++k) refs[n++] = l->operands[k].ref;
+        for (k = 0; k < l->n_outputs; ++k) refs[n++] = l->outputs[k];
+        if (l->has_absmax) refs[n++] = l->absmax_out;
+    } else if (l->kind == M3C_LAUNCH_VERIFY) {
+        for (k = 0; k < (int)M3_GRAPH_NODE_INPUT_CAPACITY; ++k) refs[n++] = l->node_in[k];
+        refs[n++] = l->row_out;
+        refs[n++] = l->row_out2;
+    } else {
+        refs[n++] = l->row_in;
+        refs[n++] = l->row_in_b;
+        refs[n++] = l->row_sum_out;
+        refs[n++] = l->row_out;
+        refs[n++] = l->row_out2;
+        refs[n++] = l->row_out3;
+        refs[n++] = l->row_out4;
+        refs[n++] = l->norm_scale;
+        refs[n++] = l->norm_bias;
+    }
+    for (i = 0U; i < n && count < capacity; ++i) {
+        if (refs[i].value != NO_VALUE) {
+            slots[count++] = plan->value_slot[refs[i].value];
+        }
+    }
+    return count;
+}
+
+/* Waves of launches that may run at the same time: only in a plan without
+ * data checks (no launch can fail, so no later launch must wait for an
+ * earlier one's verdict), a launch joins the wave before it when it shares
+ * no slot with any launch of that wave. */
+static m3_status plan_waves(m3c_plan *plan, m3_error *error)
+{
+    enum { CAP = 32 };
+    size_t wave_start = 0U;
+    size_t i;
+
+    plan->launch_wave = calloc(plan->launch_count ? plan->launch_count : 1U,
+                               sizeof(uint32_t));
+    if (plan->launch_wave == NULL) {
+        return m3c_error_set(error, M3_STATUS_OUT_OF_MEMORY,
+                             "cannot allocate the launch waves");
+    }
+    for (i = 1U; i < plan->launch_count; ++i) {
+        size_t mine[CAP];
+        size_t mine_count = launch_slots(plan, &plan->launches[i], mine, CAP);
+        bool independent = plan->flip_count == 0U &&
+                           i - wave_start <= M3C_SIDE_STREAMS;
+        size_t j;
+
+        for (j = wave_start; j < i && independent; ++j) {
+            size_t theirs[CAP];
+            size_t theirs_count = launch_slots(plan, &plan->launches[j], theirs, CAP);
+            size_t a;
+            size_t b;
+
+            for (a = 0U; a < mine_count && independent; ++a) {
+                for (b = 0U; b < theirs_count; ++b) {
+                    if (mine[a] == theirs[b]) {
+                        independent = false;
+                        break;
+                    }
+                }
+            }
+        }
+        plan->launch_wave[i] = plan->launch_wave[i - 1U];
+        if (!independent) {
+            ++plan->launch_wave[i];
+            wave_start = i;
+        }
+    }
+    return M3_STATUS_OK;
+}
+
 m3_status m3c_plan_build(const m3_graph *graph, bool fuse_enabled,
                          m3c_plan *plan, m3_error *error)
 {
@@ -1585,6 +1672,9 @@ m3_status m3c_plan_build(const m3_graph *graph, bool fuse_enabled,
         return status;
     }
     status = mark_needed_slots(graph, plan, error);
+    if (status == M3_STATUS_OK) {
+        status = plan_waves(plan, error);
+    }
     if (status != M3_STATUS_OK) {
         m3c_plan_free(plan);
         return status;

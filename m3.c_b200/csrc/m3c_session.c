@@ -35,10 +35,6 @@ typedef struct {
     size_t slot_b;
 } session_event;
 
-/* Launches of one run that may execute at the same time: up to
- * 1 + M3C_SIDE_STREAMS per wave. */
-#define M3C_SIDE_STREAMS 3
-
 /* A captured sequence of `runs` runs with slots swap_a/swap_b exchanged
  * between consecutive runs (SIZE_MAX: none), valid for the buffer assignment
  * it was captured from (kernel parameters hold buffer addresses). */
@@ -108,10 +104,8 @@ struct m3_session {
     host_pipe pipe;
     /* this rank's share of a sharded session (NULL: not sharded) */
     m3c_shard *shard;
-    /* concurrent launches: wave_join[i] is true when launch i runs beside
-     * the launches before it in its wave (independent slots, no data check
-     * before it in the run); side streams and fork/join events */
-    bool *wave_join;
+    /* concurrent launches (the plan's waves): side streams and fork/join
+     * events */
     cudaStream_t side[M3C_SIDE_STREAMS];
     cudaEvent_t fork_event;
     cudaEvent_t join_event[M3C_SIDE_STREAMS];
@@ -259,7 +253,6 @@ void m3_session_free(m3_session *session)
     if (session->fork_event != NULL) {
         (void)cudaEventDestroy(session->fork_event);
     }
-    free(session->wave_join);
     if (session->own_stream && session->stream != NULL) {
         (void)cudaStreamDestroy(session->stream);
     }
@@ -347,114 +340,34 @@ static void build_templates(m3_session *s)
     }
 }
 
-/* Slots a launch reads or writes (both buffers of a slot count as one). */
-static size_t launch_slots(const m3c_plan *plan, const m3c_launch *l,
-                           size_t *slots, size_t capacity)
+/* The side streams and events of the plan's widest wave. */
+static m3_status prepare_waves(m3_session *s, m3_error *error)
 {
-    m3c_ref refs[M3C_EW_MAX_OPERANDS + M3C_EW_MAX_OUTPUTS + 12];
-    size_t n = 0U;
-    size_t count = 0U;
-    size_t i;
-    int k;
-
-    if (l->kind == M3C_LAUNCH_EW) {
-        for (k = 0; k < l->n_operands; ++k) refs[n++] = l->operands[k].ref;
-        for (k = 0; k < l->n_outputs; ++k) refs[n++] = l->outputs[k];
-        if (l->has_absmax) refs[n++] = l->absmax_out;
-    } else if (l->kind == M3C_LAUNCH_VERIFY) {
-        for (k = 0; k < (int)M3_GRAPH_NODE_INPUT_CAPACITY; ++k) refs[n++] = l->node_in[k];
-        refs[n++] = l->row_out;
-        refs[n++] = l->row_out2;
-    } else {
-        refs[n++] = l->row_in;
-        refs[n++] = l->row_in_b;
-        refs[n++] = l->row_sum_out;
-        refs[n++] = l->row_out;
-        refs[n++] = l->row_out2;
-        refs[n++] = l->row_out3;
-        refs[n++] = l->row_out4;
-        refs[n++] = l->norm_scale;
-        refs[n++] = l->norm_bias;
-    }
-    for (i = 0U; i < n && count < capacity; ++i) {
-        if (refs[i].value != UINT32_MAX) {
-            slots[count++] = plan->value_slot[refs[i].value];
-        }
-    }
-    return count;
-}
-
-/* Waves of launches that may run at the same time: only in a plan without
- * data checks (no launch can fail, so no later launch must wait for an
- * earlier one's verdict), a launch joins the wave before it when it shares
- * no slot with any launch of that wave. */
-static m3_status plan_waves(m3_session *s, m3_error *error)
-{
-    size_t n = s->plan.launch_count;
-    size_t wave_start = 0U;
-    size_t i;
+    const uint32_t *wave = s->plan.launch_wave;
+    cudaError_t code = cudaSuccess;
     size_t widest = 0U;
-    enum { CAP = 32 };
+    size_t beside = 0U;
+    size_t i;
 
-    if (n < 2U || s->plan.flip_count != 0U) {
-        return M3_STATUS_OK;
-    }
-    s->wave_join = calloc(n, sizeof(bool));
-    if (s->wave_join == NULL) {
-        return m3c_error_set(error, M3_STATUS_OUT_OF_MEMORY,
-                             "cannot allocate the launch waves");
-    }
-    for (i = 1U; i < n; ++i) {
-        size_t mine[CAP];
-        size_t mine_count = launch_slots(&s->plan, &s->plan.launches[i], mine, CAP);
-        bool independent = i - wave_start <= M3C_SIDE_STREAMS;
-        size_t j;
-
-        for (j = wave_start; j < i && independent; ++j) {
-            size_t theirs[CAP];
-            size_t theirs_count = launch_slots(&s->plan, &s->plan.launches[j], theirs, CAP);
-            size_t a;
-            size_t b;
-
-            for (a = 0U; a < mine_count && independent; ++a) {
-                for (b = 0U; b < theirs_count; ++b) {
-                    if (mine[a] == theirs[b]) {
-                        independent = false;
-                        break;
-                    }
-                }
-            }
-        }
-        if (independent) {
-            s->wave_join[i] = true;
-            if (i - wave_start > widest) {
-                widest = i - wave_start;
-            }
-        } else {
-            wave_start = i;
+    for (i = 1U; i < s->plan.launch_count; ++i) {
+        beside = wave[i] == wave[i - 1U] ? beside + 1U : 0U;
+        if (beside > widest) {
+            widest = beside;
         }
     }
-    if (widest == 0U) {
-        free(s->wave_join);
-        s->wave_join = NULL;
-        return M3_STATUS_OK;
+    if (widest != 0U) {
+        code = cudaEventCreateWithFlags(&s->fork_event, cudaEventDisableTiming);
     }
-    {
-        cudaError_t code = cudaEventCreateWithFlags(&s->fork_event,
-                                                    cudaEventDisableTiming);
-
-        for (i = 0U; code == cudaSuccess && i < widest; ++i) {
-            code = cudaStreamCreateWithFlags(&s->side[i], cudaStreamNonBlocking);
-            if (code == cudaSuccess) {
-                code = cudaEventCreateWithFlags(&s->join_event[i],
-                                                cudaEventDisableTiming);
-            }
-        }
-        if (code != cudaSuccess) {
-            return cuda_failure(error, code, "cannot create side streams");
+    for (i = 0U; code == cudaSuccess && i < widest; ++i) {
+        code = cudaStreamCreateWithFlags(&s->side[i], cudaStreamNonBlocking);
+        if (code == cudaSuccess) {
+            code = cudaEventCreateWithFlags(&s->join_event[i],
+                                            cudaEventDisableTiming);
         }
     }
-    return M3_STATUS_OK;
+    return code == cudaSuccess
+               ? M3_STATUS_OK
+               : cuda_failure(error, code, "cannot create side streams");
 }
 
 m3_status m3_cuda_session_create(m3_session **session_output,
@@ -625,7 +538,7 @@ m3_status m3_cuda_session_create(m3_session **session_output,
         return cuda_failure(error, code, "cannot initialise session memory");
     }
     build_templates(s);
-    status = plan_waves(s, error);
+    status = prepare_waves(s, error);
     if (status != M3_STATUS_OK) {
         m3_session_free(s);
         return status;
@@ -876,8 +789,8 @@ static int launch_run(m3_session *s)
         size_t k;
         cudaError_t code;
 
-        while (s->wave_join != NULL && end < s->plan.launch_count &&
-               s->wave_join[end]) {
+        while (end < s->plan.launch_count &&
+               s->plan.launch_wave[end] == s->plan.launch_wave[i]) {
             ++end;
         }
         if (end == i + 1U) {
@@ -1850,6 +1763,39 @@ m3_status m3_cuda_graph_plan(const m3_graph *graph,
         info->allocated_bytes = plan.allocated_bytes;
     }
     fill_report(&plan, report, text, text_capacity);
+    m3c_plan_free(&plan);
+    m3_error_reset(error);
+    return M3_STATUS_OK;
+}
+
+m3_status m3_cuda_graph_waves(const m3_graph *graph,
+                              const m3_cuda_session_options *cuda,
+                              uint32_t *waves, size_t capacity,
+                              size_t *launch_count, m3_error *error)
+{
+    m3_cuda_session_options options;
+    m3c_plan plan;
+    m3_status status;
+    size_t i;
+
+    m3_cuda_session_options_init(&options);
+    if (cuda != NULL) {
+        options = *cuda;
+    }
+    if (waves == NULL && capacity != 0U) {
+        return m3c_error_set(error, M3_STATUS_INVALID_ARGUMENT,
+                             "wave output is required");
+    }
+    status = m3c_plan_build(graph, options.fuse, &plan, error);
+    if (status != M3_STATUS_OK) {
+        return status;
+    }
+    for (i = 0U; i < plan.launch_count && i < capacity; ++i) {
+        waves[i] = plan.launch_wave[i];
+    }
+    if (launch_count != NULL) {
+        *launch_count = plan.launch_count;
+    }
     m3c_plan_free(&plan);
     m3_error_reset(error);
     return M3_STATUS_OK;

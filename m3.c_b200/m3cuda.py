@@ -384,6 +384,10 @@ _CUDA_SIGNATURES = {
         ctypes.c_void_p, ctypes.POINTER(CudaSessionOptions),
         ctypes.POINTER(PlanInfo), ctypes.POINTER(PlanReport), ctypes.c_char_p,
         ctypes.c_size_t, ctypes.POINTER(M3Error)]),
+    "m3_cuda_graph_waves": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.POINTER(CudaSessionOptions),
+        ctypes.POINTER(ctypes.c_uint32), ctypes.c_size_t,
+        ctypes.POINTER(ctypes.c_size_t), ctypes.POINTER(M3Error)]),
     "m3_cuda_backend_context_create": (ctypes.c_int, [
         ctypes.POINTER(BackendOptions), ctypes.POINTER(ctypes.c_void_p),
         ctypes.POINTER(M3Error)]),
@@ -864,6 +868,23 @@ def graph_plan(graph: Graph, fuse: bool = True):
                                  ctypes.byref(info), ctypes.byref(report),
                                  text, len(text), ctypes.byref(err)), err)
     return info, report, text.value.decode()
+
+
+def graph_waves(graph: Graph, fuse: bool = True) -> list[int]:
+    """The wave of each launch of the plan: those of one wave run at the same
+    time (host only)."""
+    lib = graph.lib
+    options = CudaSessionOptions()
+    lib.m3_cuda_session_options_init(ctypes.byref(options))
+    options.fuse = fuse
+    count = ctypes.c_size_t()
+    err = M3Error()
+    check(lib.m3_cuda_graph_waves(graph.handle, ctypes.byref(options), None, 0,
+                                  ctypes.byref(count), ctypes.byref(err)), err)
+    waves = (ctypes.c_uint32 * max(count.value, 1))()
+    check(lib.m3_cuda_graph_waves(graph.handle, ctypes.byref(options), waves,
+                                  count.value, None, ctypes.byref(err)), err)
+    return list(waves[:count.value])
 
 
 def fill_uniform(seed: int, sequence: int, low: float, high: float,
