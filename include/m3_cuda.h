@@ -1091,8 +1091,11 @@ m3_status m3_cuda_cache_device_pointers(const m3_cuda_cache *cache,
  * elsewhere.
  *
  * Row strides let a padded vocabulary be named as it lies; all other arrays
- * are dense.  Only what the rule needs is read: the drafts up to the first
- * rejection, then one row of each model.
+ * are dense.  What the rule does not need has no effect, but may be read, and so
+ * must be readable and not be written meanwhile: every length, drafted token and
+ * uniform, and the probabilities of a sequence's drafted tokens up to its length
+ * also behind a rejection.  Rows at or behind the length are read in one case
+ * alone: the target's row `length` where every draft was accepted.
  *
  * One bad sequence does not fail its batch: a sequence whose length is outside
  * [0, drafts] (e.g. -1 for a padded place), or that needs a token outside the

@@ -95,18 +95,18 @@ __device__ __forceinline__ int accepted_drafts(const m3c_verify_params &p, uint6
         if (i < most) {
             const int64_t d = p.draft_tokens[b * p.drafts + i];
             const float u = uniforms[i];
-            bad = d < 0 || d >= p.vocabulary || !(u >= 0.0f && u < 1.0f);
-            if (!bad) {
-                const float t = load_element(p.target, p.dtype, (b * (p.drafts + 1u) + i) * p.target_stride + d);
-                const float q = p.draft == nullptr
-                                    ? 1.0f
-                                    : load_element(p.draft, p.dtype, (b * p.drafts + i) * p.draft_stride + d);
-                bad = !valid_probability(t) || !valid_probability(q);
-                refused = !(static_cast<double>(u) * static_cast<double>(q) < static_cast<double>(t));
+            // behind the sequence's drafts nothing counts, and no row is read
+            if (i < length) {
+                bad = d < 0 || d >= p.vocabulary || !(u >= 0.0f && u < 1.0f);
+                if (!bad) {
+                    const float t = load_element(p.target, p.dtype, (b * (p.drafts + 1u) + i) * p.target_stride + d);
+                    const float q = p.draft == nullptr
+                                        ? 1.0f
+                                        : load_element(p.draft, p.dtype, (b * p.drafts + i) * p.draft_stride + d);
+                    bad = !valid_probability(t) || !valid_probability(q);
+                    refused = !(static_cast<double>(u) * static_cast<double>(q) < static_cast<double>(t));
+                }
             }
-            // behind the sequence's drafts nothing counts
-            bad = bad && i < length;
-            refused = refused && i < length;
         }
         if (bad_sequence || i0 >= length) break;
         const uint32_t stop = __ballot_sync(0xffffffffu, bad || refused);

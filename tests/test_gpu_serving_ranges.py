@@ -14,7 +14,7 @@ import sys
 import numpy as np
 import pytest
 
-from test_gpu_serving import (TINY, U, cache_rows, device_view, e4m3_table, host, nearest_e4m3, run_norm,
+from test_gpu_serving import (TINY, U, cache_rows, device_view, e4m3_table, host, nearest_e4m3, run_norm, run_verify,
                               torch_dtype)
 
 pytestmark = pytest.mark.gpu
@@ -208,3 +208,31 @@ def test_norm_millions_of_elements_a_row(m3, gpu):
     assert abs(host(scales)[0, 0] - scale) <= slack * scale
     got = e4m3_table()[codes.cpu().numpy()]
     assert np.array_equal(got, nearest_e4m3(y / scale))
+
+
+@pytest.mark.parametrize("dtype, drawn", [("f32", True), ("bf16", True), ("bf16", False)])
+def test_verify_what_lies_behind_a_length(m3, gpu, dtype, drawn):
+    """Tokens, uniforms and rows behind a sequence's drafts have no effect, whatever they hold."""
+    import torch
+
+    batch, drafts, vocabulary = 40, 37, 500
+    g = torch.Generator(device="cuda").manual_seed(21)
+    target = torch.softmax(2 * torch.randn(batch, drafts + 1, vocabulary, generator=g, device="cuda"), -1)
+    target = target.to(torch_dtype(dtype))
+    draft = target[:, :drafts].clone() if drawn else None
+    drafted = target[:, :drafts].float().argmax(-1).int()
+    uniforms = torch.rand(batch, drafts + 1, generator=g, device="cuda")
+    uniforms[:, :drafts] *= 0.1
+    lengths = (torch.arange(batch, device="cuda") % (drafts + 1)).int()
+    clean = run_verify(m3, target, draft, drafted, lengths, uniforms)
+    behind = torch.arange(drafts + 1, device="cuda")[None] >= lengths[:, None]
+    target[behind & (torch.arange(drafts + 1, device="cuda")[None] > lengths[:, None])] = float("nan")
+    drafted[behind[:, :drafts]] = -5
+    uniforms[:, :drafts][behind[:, :drafts]] = 9.0
+    if drawn:
+        draft[behind[:, :drafts]] = float("nan")
+    again = run_verify(m3, target, draft, drafted, lengths, uniforms)
+    assert np.array_equal(clean[0], again[0]) and np.array_equal(clean[1], again[1])
+    assert np.all(clean[1] >= 0)
+    # draws from the draft model (here the target) are all accepted, given drafts as often as the target has them
+    assert not drawn or clean[1].max() > 32
