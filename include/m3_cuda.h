@@ -1085,8 +1085,9 @@ m3_status m3_cuda_cache_device_pointers(const m3_cuda_cache *cache,
  * behind the m accepted ones with uniforms[drafts]: from max(target_m -
  * draft_m, 0) after a rejection (from target_m where that is zero for every
  * token), from target_m where all drafts were accepted.  The drawn token is
- * the first whose running sum of weights exceeds uniform * total, the sums in
- * 64 bits.  So the tokens are distributed as the target's own.  Without
+ * the first whose running sum of weights exceeds uniform * total, each sum to
+ * within 2^-44 of the total (64-bit sums; what the F32 differences lose joins
+ * them in F32 sums of eight).  So the tokens are distributed as the target's own.  Without
  * `draft` the drafts were not drawn but given: draft_i is 1 at token_i and 0
  * elsewhere.
  *
