@@ -1039,15 +1039,18 @@ typedef struct {
 typedef struct {
     void *data;
     m3_dtype dtype;              /* F32, F16 or BF16 */
-    uint64_t token_stride;       /* elements (0: heads * head_dim) */
-    uint64_t head_stride;        /* elements (0: head_dim) */
+    uint64_t token_stride;       /* elements, at least head_dim (0: heads *
+                                    head_dim); either stride may be the outer */
+    uint64_t head_stride;        /* elements, at least head_dim (0: head_dim) */
 } m3_cuda_cache_rows;
 
 /* Quantise the rows' keys and values into their slots; each vector of head_dim
  * elements is one group.  No two rows of a call may name one slot, nor may
  * calls that overlap in time name a slot that one of them writes: its vectors
  * are then unspecified (all other slots hold what they should).  The rows'
- * own vectors may overlap (they are only read). */
+ * own vectors may overlap (they are only read).  Neither they nor the batch's
+ * arrays may lie in the cache's own memory (M3_STATUS_INVALID_ARGUMENT; the
+ * byte spans are compared). */
 m3_status m3_cuda_cache_write(m3_cuda_cache *cache, void *stream,
                               const m3_cuda_cache_batch *batch,
                               const m3_cuda_cache_rows *keys,
@@ -1056,7 +1059,8 @@ m3_status m3_cuda_cache_write(m3_cuda_cache *cache, void *stream,
 /* Read the rows' slots back: code * scale, in F32, rounded to the rows' dtype.
  * Several rows may name one slot (a shared prefix).  No two vectors of `keys`
  * and `values` may overlap (they may interleave): what overlaps is then
- * unspecified. */
+ * unspecified.  Their spans may overlap neither the batch's arrays nor the
+ * cache's own memory (M3_STATUS_INVALID_ARGUMENT). */
 m3_status m3_cuda_cache_read(m3_cuda_cache *cache, void *stream,
                              const m3_cuda_cache_batch *batch,
                              const m3_cuda_cache_rows *keys,

@@ -13,6 +13,7 @@ struct m3_cuda_cache {
     m3_cuda_cache_options options;
     int device;
     unsigned char *arena;
+    size_t arena_bytes;
     uint8_t *codes[2];
     float *scales[2];
     unsigned long long *first_skipped;   /* device; the word behind it holds
@@ -342,8 +343,8 @@ m3_status m3_cuda_cache_create(m3_cuda_cache **cache,
         free(c);
         return status;
     }
-    code = cudaMalloc((void **)&c->arena, 2U * (code_bytes + scale_bytes) +
-                                              M3C_ARENA_ALIGNMENT);
+    c->arena_bytes = 2U * (code_bytes + scale_bytes) + M3C_ARENA_ALIGNMENT;
+    code = cudaMalloc((void **)&c->arena, c->arena_bytes);
     if (code == cudaSuccess) {
         c->codes[0] = c->arena;
         c->codes[1] = c->codes[0] + code_bytes;
@@ -415,16 +416,61 @@ m3_status m3_cuda_cache_device_pointers(const m3_cuda_cache *cache,
     return M3_STATUS_OK;
 }
 
-/* The launch block of one write or read, checked. */
+/* The span of a batch's keys or values, and their strides: `vectors` steps from
+ * head to head, `tokens` from token to token.  Either may be the outer one. */
+static m3_status cache_span(const m3_cuda_cache *cache,
+                            const m3_cuda_cache_rows *r, const char *name,
+                            uint64_t rows, span *tokens, span *vectors,
+                            m3_error *error)
+{
+    uint64_t heads = rows == 0U ? 0U : cache->options.heads;
+    uint64_t dim = cache->options.head_dim;
+    uint64_t size;
+    uint64_t other_heads;
+    m3_status status = check_float(r->dtype, name, error);
+
+    if (status != M3_STATUS_OK) {
+        return status;
+    }
+    size = m3c_dtype_size(r->dtype);
+    status = rows_span(vectors, name, r->data, heads, dim, r->head_stride,
+                       size, error);
+    if (status == M3_STATUS_OK) {
+        status = rows_span(tokens, name, r->data, rows, dim,
+                           r->token_stride == 0U
+                               ? cache->options.heads * dim
+                               : r->token_stride,
+                           size, error);
+    }
+    if (status != M3_STATUS_OK || rows == 0U) {
+        return status;
+    }
+    /* from the last token's first vector to its last */
+    other_heads = vectors->end - vectors->begin - dim * size;
+    if (other_heads > UINTPTR_MAX - tokens->end) {
+        return m3c_error_set(error, M3_STATUS_OVERFLOW, "%s size overflows",
+                             name);
+    }
+    tokens->end += other_heads;
+    return M3_STATUS_OK;
+}
+
+/* The launch block of one write, or read (`into_rows`), checked. */
 static m3_status cache_params(const m3_cuda_cache *cache,
                               const m3_cuda_cache_batch *batch,
                               const m3_cuda_cache_rows *const rows[2],
-                              m3c_cache_params *p, m3_error *error)
+                              bool into_rows, m3c_cache_params *p,
+                              m3_error *error)
 {
-    static const char *const names[2] = {"cache keys", "cache values"};
-    uint64_t heads;
-    uint64_t dim;
+    enum { KEYS, VALUES, PAGE_TABLE, OFFSETS, STARTS, SPANS };
+    static const char *const names[SPANS] = {
+        "cache keys", "cache values", "cache page table", "cache offsets",
+        "cache starts"};
+    span s[SPANS];
+    span memory;
+    m3_status status = M3_STATUS_OK;
     int k;
+    int other;
 
     if (cache == NULL || batch == NULL || rows[0] == NULL || rows[1] == NULL) {
         return m3c_error_set(error, M3_STATUS_INVALID_ARGUMENT,
@@ -437,62 +483,54 @@ static m3_status cache_params(const m3_cuda_cache *cache,
                              "cache batch has too many rows, sequences or "
                              "pages");
     }
-    heads = cache->options.heads;
-    dim = cache->options.head_dim;
     memset(p, 0, sizeof(*p));
-    for (k = 0; k < 2; ++k) {
-        const m3_cuda_cache_rows *r = rows[k];
+    memset(s, 0, sizeof(s));
+    for (k = KEYS; k <= VALUES; ++k) {
         span vectors;
-        span tokens;
-        m3_status status = check_float(r->dtype, names[k], error);
 
-        /* a token's vectors, then the tokens */
-        if (status == M3_STATUS_OK) {
-            status = rows_span(&vectors, names[k], r->data,
-                               batch->rows == 0U ? 0U : heads, dim,
-                               r->head_stride, m3c_dtype_size(r->dtype), error);
-        }
-        if (status == M3_STATUS_OK) {
-            uint64_t extent = batch->rows == 0U
-                                  ? 0U
-                                  : (heads - 1U) * vectors.stride + dim;
-
-            /* a token's rows may interleave with the next token's (heads
-             * outermost): only the last address must not overflow */
-            status = rows_span(&tokens, names[k], r->data,
-                               batch->rows, extent,
-                               r->token_stride == 0U ? heads * dim
-                               : r->token_stride < extent && r->token_stride >= dim
-                                   ? extent
-                                   : r->token_stride,
-                               m3c_dtype_size(r->dtype), error);
-        }
+        status = cache_span(cache, rows[k], names[k], batch->rows, &s[k],
+                            &vectors, error);
         if (status != M3_STATUS_OK) {
             return status;
         }
         p->codes[k] = cache->codes[k];
         p->scales[k] = cache->scales[k];
-        p->rows[k] = r->data;
-        p->dtype[k] = (int32_t)r->dtype;
-        p->token_stride[k] = r->token_stride == 0U ? heads * dim
-                                                   : r->token_stride;
+        p->rows[k] = rows[k]->data;
+        p->dtype[k] = (int32_t)rows[k]->dtype;
+        p->token_stride[k] = s[k].stride;
         p->head_stride[k] = vectors.stride;
     }
     if (batch->rows != 0U && batch->sequences != 0U) {
-        static const char *const arrays[3] = {
-            "cache page table", "cache offsets", "cache starts"};
-        const void *data[3];
+        const void *data[SPANS] = {NULL, NULL, batch->page_table,
+                                   batch->offsets, batch->starts};
+        const uint64_t count[SPANS] = {
+            0U, 0U, batch->sequences * batch->page_table_stride,
+            batch->sequences + 1U, batch->starts == NULL ? 0U : batch->sequences};
 
-        data[0] = batch->page_table;
-        data[1] = batch->offsets;
-        data[2] = batch->starts;
-        for (k = 0; k < 3; ++k) {
-            if ((data[k] == NULL && k < 2 &&
-                 (k != 0 || batch->page_table_stride != 0U)) ||
+        memory.name = "the cache's memory";
+        memory.begin = (uintptr_t)cache->arena;
+        memory.end = memory.begin + cache->arena_bytes;
+        for (k = PAGE_TABLE; k < SPANS; ++k) {
+            if ((data[k] == NULL && count[k] != 0U) ||
                 (uintptr_t)data[k] % sizeof(int32_t) != 0U) {
                 return m3c_error_set(error, M3_STATUS_INVALID_ARGUMENT,
-                                     "%s is absent or not aligned", arrays[k]);
+                                     "%s is absent or not aligned", names[k]);
             }
+            status = rows_span(&s[k], names[k], data[k], 1U, count[k], 0U,
+                               sizeof(int32_t), error);
+            if (status != M3_STATUS_OK) {
+                return status;
+            }
+        }
+        for (k = KEYS; status == M3_STATUS_OK && k < SPANS; ++k) {
+            status = check_apart(&s[k], &memory, error);
+            for (other = PAGE_TABLE; status == M3_STATUS_OK && into_rows &&
+                                     k <= VALUES && other < SPANS; ++other) {
+                status = check_apart(&s[k], &s[other], error);
+            }
+        }
+        if (status != M3_STATUS_OK) {
+            return status;
         }
     }
     p->page_table = batch->page_table;
@@ -513,8 +551,7 @@ static m3_status cache_move(m3_cuda_cache *cache, void *stream,
                             const m3_cuda_cache_batch *batch,
                             const m3_cuda_cache_rows *keys,
                             const m3_cuda_cache_rows *values,
-                            int (*launch)(const m3c_cache_params *, void *),
-                            m3_error *error)
+                            bool into_rows, m3_error *error)
 {
     const m3_cuda_cache_rows *rows[2];
     m3c_cache_params p;
@@ -523,7 +560,7 @@ static m3_status cache_move(m3_cuda_cache *cache, void *stream,
 
     rows[0] = keys;
     rows[1] = values;
-    status = cache_params(cache, batch, rows, &p, error);
+    status = cache_params(cache, batch, rows, into_rows, &p, error);
     if (status != M3_STATUS_OK) {
         return status;
     }
@@ -535,7 +572,9 @@ static m3_status cache_move(m3_cuda_cache *cache, void *stream,
     if (status != M3_STATUS_OK) {
         return status;
     }
-    status = launched(launch(&p, stream), error);
+    status = launched(into_rows ? m3c_launch_cache_read(&p, stream)
+                                : m3c_launch_cache_write(&p, stream),
+                      error);
     leave_device(cache->device, previous);
     return status;
 }
@@ -546,8 +585,7 @@ m3_status m3_cuda_cache_write(m3_cuda_cache *cache, void *stream,
                               const m3_cuda_cache_rows *values,
                               m3_error *error)
 {
-    return cache_move(cache, stream, batch, keys, values,
-                      m3c_launch_cache_write, error);
+    return cache_move(cache, stream, batch, keys, values, false, error);
 }
 
 m3_status m3_cuda_cache_read(m3_cuda_cache *cache, void *stream,
@@ -556,8 +594,7 @@ m3_status m3_cuda_cache_read(m3_cuda_cache *cache, void *stream,
                              const m3_cuda_cache_rows *values,
                              m3_error *error)
 {
-    return cache_move(cache, stream, batch, keys, values,
-                      m3c_launch_cache_read, error);
+    return cache_move(cache, stream, batch, keys, values, true, error);
 }
 
 m3_status m3_cuda_cache_synchronize(m3_cuda_cache *cache, void *stream,

@@ -236,3 +236,66 @@ def test_verify_what_lies_behind_a_length(m3, gpu, dtype, drawn):
     assert np.all(clean[1] >= 0)
     # draws from the draft model (here the target) are all accepted, given drafts as often as the target has them
     assert not drawn or clean[1].max() > 32
+
+
+def test_cache_overlaps_are_refused(m3, gpu):
+    """Rows that a read would write over the batch's arrays, and anything in the cache's own memory."""
+    import torch
+
+    c = m3.Cache(4, 16, 2, 64)
+    ints = torch.zeros(64, dtype=torch.int32, device="cuda")
+    data = torch.full((8, 2, 64), 3.0, device="cuda")
+    other = torch.full((8, 2, 64), 3.0, device="cuda")
+    ints[17] = 4                                    # offsets 0, 4
+
+    def batch(**change):
+        fields = dict(page_table=ints.data_ptr(), page_table_stride=2, offsets=ints.data_ptr() + 64,
+                      starts=ints.data_ptr() + 128, sequences=1, rows=4)
+        fields.update(change)
+        return m3.CacheBatch(**fields)
+
+    def at(pointer, token_stride=128, head_stride=64):
+        return m3.CacheRows(data=pointer, dtype=m3.F32, token_stride=token_stride, head_stride=head_stride)
+
+    fine, second = cache_rows(m3, data), cache_rows(m3, other)
+    inside = data.data_ptr()
+    end = inside + 4 * 128 * 4                      # of the four rows
+    memory = c.pointers()
+    refusals = []
+    for k, name in ((0, "keys"), (1, "values")):
+        pair = [second, second]
+        pair[k] = fine
+        for array, change in (("page table", dict(page_table=inside)), ("offsets", dict(offsets=end - 4)),
+                              ("starts", dict(starts=inside + 1000)), ("page table", dict(page_table=inside - 4))):
+            refusals.append((c.read, batch(**change), pair, f"cache {name} overlaps cache {array}"))
+        for call in (c.write, c.read):
+            pair = [second, second]
+            pair[k] = at(memory[3 * k] + 256)       # the keys' codes, the values' scales
+            refusals.append((call, batch(), pair, f"cache {name} overlaps the cache's memory"))
+    for call in (c.write, c.read):
+        for array, change in (("page table", dict(page_table=memory[0])), ("offsets", dict(offsets=memory[1])),
+                              ("starts", dict(starts=memory[3]))):
+            refusals.append((call, batch(**change), [fine, second], f"cache {array} overlaps the cache's memory"))
+        # from below the cache into it, by the last vector
+        low = at(memory[0] - 4 * (3 * 128 + 64 + 64) + 4)
+        refusals.append((call, batch(), [low, second], "cache keys overlaps the cache's memory"))
+        low = at(memory[0] - 4 * (3 * 64 + 512 + 64) + 4, 64, 512)
+        refusals.append((call, batch(), [second, low], "cache values overlaps the cache's memory"))
+    for call, b, pair, text in refusals:
+        with pytest.raises(m3.M3Failure) as failure:
+            call(b, *pair)
+        assert failure.value.status == m3.INVALID_ARGUMENT and failure.value.message == text
+    c.synchronize()
+    assert bool((data == 3.0).all()) and not any(ints[18:].tolist())
+    # arrays next to the rows, and between the tokens of rows that lie heads first
+    c.write(batch(page_table=ints.data_ptr(), starts=None), fine, second)
+    wide = torch.full((2, 8, 64), 3.0, device="cuda")
+    heads_first = at(wide.data_ptr(), 64, 512)
+    around = torch.full((4 * 128 + 16,), 0.0, device="cuda")
+    c.write(batch(page_table=around.data_ptr() + 4 * 512), at(around.data_ptr()), second)
+    c.read(batch(page_table=around.data_ptr() + 4 * 512), at(around.data_ptr()), heads_first)
+    # what a write reads may be shared: zeros are a table, offsets of nothing, and numbers
+    zeros = torch.zeros(8, 2, 64, device="cuda")
+    c.write(batch(page_table=zeros.data_ptr(), offsets=zeros.data_ptr()), cache_rows(m3, zeros), second)
+    c.synchronize()
+    assert bool((wide[:, :4] != 3.0).sum() == 0) and bool((wide[:, 4:] == 3.0).all())
