@@ -672,33 +672,33 @@ int norm_launch(const m3c_norm_e4m3_params &p, cudaStream_t stream)
 template <int DT, int MODE>
 int norm_depth(const m3c_norm_e4m3_params &p, bool vectors, bool wide, cudaStream_t stream)
 {
+    // pieces per thread.  What a thread does once per row (the root, the divisor)
+    // weighs on one piece: many rows of one group take two of 16 elements (16384 x
+    // 4096 bf16 without residual: a tenth less time).  With a divisor per piece, or
+    // too few rows to fill the SMs with a row's fewer threads, one is faster.  Rows
+    // past 8192 elements need four
+    const bool many = p.rows >= 2048u && MODE == GROUP_ROW;
     if constexpr (DT != M3C_F32) {
-        // pieces per thread.  What a thread does once per row (the root, the
-        // divisor) weighs on one piece: many rows of one group take two (16384 x
-        // 4096 bf16 without residual: a tenth less time).  With a divisor per
-        // piece, or too few rows to fill the SMs with a row's fewer threads, one
-        // is faster.  Rows past 8192 elements need four
         const uint64_t pieces = p.width / 16u;
-        const bool many = p.rows >= 2048u && MODE == GROUP_ROW;
-        if (wide) {
-            if (pieces <= 512u && !(many && pieces > 32u)) return norm_launch<DT, MODE, 16, 1>(p, stream);
-            if (pieces <= 512u) return norm_launch<DT, MODE, 16, 2>(p, stream);
-            return norm_launch<DT, MODE, 16, 4>(p, stream);
+        if (wide && pieces > 512u) return norm_launch<DT, MODE, 16, 4>(p, stream);
+        if constexpr (MODE == GROUP_ROW) {
+            if (wide && many && pieces > 32u) return norm_launch<DT, MODE, 16, 2>(p, stream);
         }
+        if (wide) return norm_launch<DT, MODE, 16, 1>(p, stream);
     }
-    // single elements: 333 rows of 2051 F32 take 5.4 us with four per thread and
+    // single elements: 333 rows of 2051 F32 take 5.3 us with four per thread and
     // 6.4 with eight, which are for the widths that four leave past 1024 threads
     if (!vectors && p.width <= 4096u) return norm_launch<DT, MODE, 1, 4>(p, stream);
     if (!vectors) return norm_launch<DT, MODE, 1, 8>(p, stream);
     // the same in pieces of eight elements, of which F32's take as many registers
-    // as 16 of the others (8192 x 4096 with residual: 70 us with two, 72 with
-    // four)
+    // as 16 of the others (8192 x 4096 with residual: 66.6 us with two)
     const uint64_t pieces = p.width / 8u;
-    const bool many = p.rows >= 2048u && MODE == GROUP_ROW && DT != M3C_F32;
     if (pieces <= 32u) return norm_launch<DT, MODE, 8, 1>(p, stream);
-    if (pieces <= 64u || (pieces <= 1024u && !many)) return norm_launch<DT, MODE, 8, 2>(p, stream);
-    if (pieces <= 1024u) return norm_launch<DT, MODE, 8, 4>(p, stream);
-    return norm_launch<DT, MODE, 8, 8>(p, stream);
+    if (pieces > 1024u) return norm_launch<DT, MODE, 8, 8>(p, stream);
+    if constexpr (DT != M3C_F32 && MODE == GROUP_ROW) {
+        if (many && pieces > 64u) return norm_launch<DT, MODE, 8, 4>(p, stream);
+    }
+    return norm_launch<DT, MODE, 8, 2>(p, stream);
 }
 
 template <int DT>
@@ -1037,9 +1037,9 @@ int cache_pieces(uint32_t dim, uint32_t vec, int most, int preferred, uint32_t *
 }
 
 // Pieces of 32 bytes (`wide`: the rows are aligned for them) unless pieces of 16
-// leave fewer lanes idle.  More than two pieces of 16 elements to write leave too
-// few threads on an SM; of one and two, one is faster (65536 rows of 8 x 128
-// written in 70.7 against 72.7 us, 262144 read in 249 against 251 us).
+// leave fewer lanes idle: one a lane up to 512 elements, for reading three beyond
+// (two are never fewer idle lanes than one, or than three).  More than one to
+// write leave too few threads on an SM.
 template <int DT, bool WRITE>
 int launch_cache_pieces(const m3c_cache_params &p, bool wide, cudaStream_t stream)
 {
@@ -1047,11 +1047,12 @@ int launch_cache_pieces(const m3c_cache_params &p, bool wide, cudaStream_t strea
     const int narrow = cache_pieces(p.head_dim, 8u, 3, 3, &idle);
     if constexpr (DT != M3C_F32) {
         uint32_t wide_idle = 0;
-        const int k = cache_pieces(p.head_dim, 16u, WRITE ? 2 : 3, 1, &wide_idle);
+        const int k = cache_pieces(p.head_dim, 16u, WRITE ? 1 : 3, 1, &wide_idle);
         if (wide && wide_idle <= idle) {
-            if (k == 1) return launch_cache_vectors<DT, 16, WRITE, 1>(p, stream);
-            if (k == 2) return launch_cache_vectors<DT, 16, WRITE, 2>(p, stream);
-            return launch_cache_vectors<DT, 16, WRITE, WRITE ? 2 : 3>(p, stream);
+            if constexpr (!WRITE) {
+                if (k == 3) return launch_cache_vectors<DT, 16, WRITE, 3>(p, stream);
+            }
+            return launch_cache_vectors<DT, 16, WRITE, 1>(p, stream);
         }
     }
     if (narrow == 1) return launch_cache_vectors<DT, 8, WRITE, 1>(p, stream);
