@@ -23,6 +23,13 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (B200)")
 
 
+def pytest_collection_modifyitems(items):
+    """Where the reference with this provider patched in could not be built, the
+    tests that need it fail: last, so that `-x` still runs all others."""
+    if not os.path.exists(os.path.join(ROOT, "integration", "_ref", "libm3ref_cuda.so")):
+        items.sort(key=lambda item: item.path.name == "test_gpu_integration.py")
+
+
 def _load(name: str, path: str):
     if name in sys.modules:
         return sys.modules[name]
