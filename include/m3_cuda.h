@@ -952,7 +952,7 @@ m3_status m3_cuda_abs_max_static(int device, void *stream, m3_dtype dtype,
  * and each `group` consecutive elements of a row of y quantised together (the
  * root is common to a row and leaves the quotients y / scale: they are taken of
  * h * scale, with two roundings fewer, but in groups where that product leaves
- * the F32 range or comes near its lower end).
+ * the F32 range or comes near its lower end; a y below 2^-126 may be 0).
  * The row sums run in F32 in a fixed order of their own (not the reference's
  * left-to-right order of M3_OP_RMS_NORM; no chain of F32 additions is longer than
  * 300), so results repeat bit for bit; a row

@@ -186,9 +186,10 @@ def test_norm_zero_rows_with_a_small_epsilon(m3, gpu):
         x = torch.zeros(3, width, device="cuda")
         x[1] = 1.0
         w = torch.ones(width, device="cuda")
-        codes, scales = run_norm(m3, x, w, group, epsilon=1e-20)
-        check_norm_ranges(x, w, group, codes, scales, 1e-20)
-        assert not bool((codes[::2] & 0x7f).any()) and np.all(host(scales[::2]) == TINY)
+        for epsilon in (1e-20, 1e-12):
+            codes, scales = run_norm(m3, x, w, group, epsilon=epsilon)
+            check_norm_ranges(x, w, group, codes, scales, epsilon)
+            assert not bool((codes[::2] & 0x7f).any()) and np.all(host(scales[::2]) == TINY)
 
 
 def test_norm_millions_of_elements_a_row(m3, gpu):
