@@ -71,7 +71,9 @@ __device__ __forceinline__ float largest_of(const float (&v)[N])
     } else {
         float m = 0.0f;
 #pragma unroll
-        for (int i = 0; i < N; i += 2) asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(m), "f"(v[i]), "f"(v[i + 1]));
+        for (int i = 0; i < N; i += 2) {
+            asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(m), "f"(v[i]), "f"(v[i + 1]));
+        }
         return m;
     }
 }

@@ -60,20 +60,21 @@ unsigned capped_grid(uint64_t wanted, unsigned per_sm)
 //   per group of y: scale, codes (m3c_e4m3.cuh).
 //
 // Bytes bound it: x and r in, h and the codes out, 7 bytes per element of a
-// 16-bit residual stream.  16384 x 4096 bf16 with residual: 69.8 us, 6.7 TB/s,
-// 1.02 of the measured copy rate, in groups of 128 too; with accesses of 16 bytes
-// 73.5 us, and 85.2 in groups, which then made a divisor per eight elements.
-// Without a residual, three bytes an element, the instructions weigh more: 44.4
-// us (0.69).  Both
-// kernels below read a row once and keep h on the SM until its codes are out.
+// 16-bit residual stream.  16384 x 4096 bf16 with residual: 70.3 us, 6.7 TB/s,
+// 1.02 of the measured copy rate (71.8 us in groups of 128, with a divisor per
+// piece).  Without a residual, three bytes an element, the instructions weigh
+// more: 43 us (0.71).  Both kernels below read a row once and keep h on the SM
+// until its codes are out.
 
 // The register kernel: `threads` threads (whole warps) own a row, each K pieces
 // of VEC consecutive elements in registers, piece k of thread i being number
 // k * threads + i of the row, so a warp reads consecutive memory: 32 bytes a lane
 // where every row is aligned for it (VEC = 16 elements of 16 bits, 8 of F32), 16
-// bytes (VEC = 8) or one element (VEC = 1) elsewhere.  z = h w is made before the row's sum is known, and the largest |y|
-// is the largest |z| times the inverse root (rounding keeps order), so one
-// exchange between a row's warps carries the sum of squares and the maximum.
+// bytes (VEC = 8) or one element (VEC = 1) elsewhere: odd widths and addresses pay
+// for it (8192 x 4099 bf16 87.6 us, 0.18 of the copy rate; with residual 140 us,
+// 0.26).  z = h w is made before the row's sum is known, and the largest |y| is the
+// largest |z| times the inverse root (rounding keeps order), so one exchange
+// between a row's warps carries the sum of squares and the maximum.
 //   GROUP_ROW    one group per row
 //   GROUP_LANES  a group is 1, 2, 4, ... or 32 pieces: the lanes that own one
 //                reduce among themselves
@@ -675,9 +676,9 @@ int norm_depth(const m3c_norm_e4m3_params &p, bool vectors, bool wide, cudaStrea
 {
     // pieces per thread.  What a thread does once per row (the root, the divisor)
     // weighs on one piece: many rows of one group take two of 16 elements (16384 x
-    // 4096 bf16 without residual: a tenth less time).  With a divisor per piece, or
-    // too few rows to fill the SMs with a row's fewer threads, one is faster.  Rows
-    // past 8192 elements need four
+    // 4096 bf16 without residual: 43 us, 50 with one).  With a divisor per piece, or
+    // too few rows to fill the SMs with a row's fewer threads, one is as fast or
+    // faster.  Rows past 8192 elements need four
     const bool many = p.rows >= 2048u && MODE == GROUP_ROW;
     if constexpr (DT != M3C_F32) {
         const uint64_t pieces = p.width / 16u;
@@ -688,7 +689,7 @@ int norm_depth(const m3c_norm_e4m3_params &p, bool vectors, bool wide, cudaStrea
         if (wide) return norm_launch<DT, MODE, 16, 1>(p, stream);
     }
     // single elements: 333 rows of 2051 F32 take 5.3 us with four per thread and
-    // 6.4 with eight, which are for the widths that four leave past 1024 threads
+    // 5.9 with eight, which are for the widths that four leave past 1024 threads
     if (!vectors && p.width <= 4096u) return norm_launch<DT, MODE, 1, 4>(p, stream);
     if (!vectors) return norm_launch<DT, MODE, 1, 8>(p, stream);
     // the same in pieces of eight elements, of which F32's take as many registers
@@ -781,10 +782,11 @@ __device__ __forceinline__ void find_slots(const m3c_cache_params &p, uint32_t f
 // takes over where a row's vectors do not fit a block.  The slots of a CTA's
 // rows are found once, in shared memory.
 //
-// Bytes bound both directions: three per element of 16-bit rows.  262144 rows
-// of 8 heads of 128 in bf16 are read in 249 us (6.5 TB/s, 1.00 of the measured
-// copy rate), 65536 written in 70.7 us (5.8 TB/s, 0.88), 16384 in 20.0 us (0.77).
-// Writing has some twelve instructions an element (the maximum over the vector,
+// Bytes bound both directions: three per element of 16-bit rows, five of F32.
+// 262144 rows of 8 heads of 128 in bf16 are read in 249 us (6.5 TB/s, 1.00 of the
+// measured copy rate), 131072 in F32 in 207 us (0.99); 65536 in bf16 are written in
+// 70.6 us (5.8 TB/s, 0.88), 16384 in 20.1 us (0.77), in F32 in 103 us (1.00) and
+// 28.4 us (0.90).  Writing has some twelve instructions an element (the maximum over the vector,
 // a correctly rounded quotient) and the dependent loads that find a slot.
 struct cache_shape {
     uint32_t lane_shift;
@@ -824,8 +826,9 @@ struct cache_place {
 };
 
 // Writing: the CTA walks over its rows, the next rows' loads on their way while
-// one row's codes are made; the slots are found behind the first loads.  (One
-// row a CTA, unrolled as reading is, took 87 us for the 65536 rows above.)
+// one row's codes are made; the slots are found behind the first loads.  Two CTAs
+// of 512 threads an SM leave 64 registers, of which three F32 pieces (heads of 96)
+// spill seven: 65536 rows of 8 x 96 take 85 us (0.91).
 template <int DT, int VEC, int P>
 __global__ void __launch_bounds__(CACHE_THREADS, 2)
     cache_write_kernel(const __grid_constant__ m3c_cache_params p, const __grid_constant__ cache_shape shape)
@@ -886,10 +889,8 @@ __global__ void __launch_bounds__(CACHE_THREADS, 2)
     }
 }
 
-// Reading: the slots first, then STEPS rows of a thread at once.  (Walking as
-// writing does took 254 us for the 262144 rows above.)  Stores of 32 bytes a lane
-// fill their sectors at once: with two of 16 bytes 131072 F32 rows took 278 us,
-// with one 207.
+// Reading: the slots first, then STEPS rows of a thread at once, with stores of 32
+// bytes a lane, which fill their sectors at once.
 template <int DT, int VEC, int P, int STEPS>
 __global__ void __launch_bounds__(CACHE_THREADS)
     cache_read_kernel(const __grid_constant__ m3c_cache_params p, const __grid_constant__ cache_shape shape)
@@ -937,7 +938,10 @@ __global__ void __launch_bounds__(CACHE_THREADS)
     }
 }
 
-// Any shape: one warp per (row, keys or values, head).
+// Any shape, and keys and values of two types: one warp per (row, keys or values,
+// head), one element a lane.  What bounds it is the search for the slot, once a
+// vector, and the narrow accesses: 16384 rows of 8 x 60 bf16 are written in 95 us
+// and read in 72 (0.08 and 0.10 of the copy rate).
 template <bool WRITE>
 __global__ void __launch_bounds__(QUANT_THREADS) cache_any_kernel(const __grid_constant__ m3c_cache_params p)
 {
@@ -1002,8 +1006,9 @@ int launch_cache_vectors(const m3c_cache_params &p, cudaStream_t stream)
         const dim3 grid((p.row_count - 1u) / (shape.rows * shape.steps) + 1u, chunks);
         cache_write_kernel<DT, VEC, P><<<grid, block, 0, stream>>>(p, shape);
     } else {
-        // a small batch takes one: the unrolled code's own fetch costs more
-        // than it hides
+        // the 262144 rows above take 297 us with one row at once; a small batch
+        // takes one all the same, since the unrolled code's own fetch costs more
+        // than it hides (500 rows of 4 x 64 F32: 2.8 us, 3.1 with four)
         constexpr int MANY = VEC * P == 8 ? 4 : 2;
         shape.steps = groups < MANY * resident ? 1u : MANY;
         const dim3 grid((p.row_count - 1u) / (shape.rows * shape.steps) + 1u, chunks);

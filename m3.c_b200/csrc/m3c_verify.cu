@@ -9,10 +9,14 @@
 // running sums are 64-bit sums, since a vocabulary of 10^5 tokens puts F32
 // rounding errors of a sum past whole tokens' probabilities.
 //
-// Bytes bound large batches (one row of each model per sequence), latency small
-// ones: 128 sequences over 131072 tokens in F32 take 28.7 us (4.7 TB/s, 0.71 of
-// the measured copy rate), one over 32000 takes 6.5 us, nearly all of it loads
-// that wait for one another.  A cluster of CTAs takes a sequence, its warps one
+// Bytes bound large batches in F32 (one row of each model per sequence), latency
+// small ones: 128 sequences over 131072 tokens in F32 take 29.0 us (4.6 TB/s, 0.70
+// of the measured copy rate), one over 32000 takes 6.6 us, nearly all of it loads
+// that wait for one another.  16-bit rows take as long for half the bytes (27.7 us,
+// 0.37; 256 sequences over 32000 tokens 17.9 us, 0.28): a lane has one load per
+// model on its way and then 16 numbers to widen, convert and add.  Rows aligned
+// for no vector are read by single elements (131073 tokens in F32: 37.8 us, 0.54).
+// A cluster of CTAs takes a sequence, its warps one
 // contiguous part of the vocabulary each.  One pass over the rows sums the
 // parts; the parts' sums go round through the CTAs' shared memory, and the CTA
 // that owns the part in which the running sum passes the aim looks for the token
@@ -452,7 +456,7 @@ int launch_verify(const m3c_verify_params &p, cudaStream_t stream)
     }
     // as many CTAs for a sequence as run at the same time (two per SM), while
     // each keeps some elements per thread.  128 sequences over 131072 tokens
-    // in F32: 28.7 us with 2 CTAs each, 31.7 with 4, 33.0 with 1
+    // in F32: 29.0 us with 2 CTAs each, 31.8 with 4, 33.2 with 1
     uint32_t ctas = VERIFY_MOST_CTAS;
     while (ctas > 1u && (p.batch * ctas > 2u * static_cast<uint64_t>(sms) ||
                          p.vocabulary < ctas * static_cast<uint32_t>(VERIFY_THREADS))) {
