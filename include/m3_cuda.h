@@ -649,7 +649,8 @@ m3_status m3_cuda_graph_waves(const m3_graph *graph,
  * replicated (broadcast constants such as a snake alpha [1,C,1] split along
  * time, a norm scale, scalars).  Row operators (SOFTMAX, TOP_K, ROW_SUM,
  * RMS_NORM, RMS_NORM_E4M3, LAYER_NORM) need the split axis to differ from
- * their input's last axis; CATEGORICAL and VERIFY_DRAFT are not split.  M3_OP_ABS_MAX is a global reduction: every rank
+ * their input's last axis; CATEGORICAL and VERIFY_DRAFT are not split.
+ * M3_OP_ABS_MAX is a global reduction: every rank
  * reduces its slab, then one NCCL all-reduce (MAX over the unsigned bit
  * patterns, exact and order-free) on the session's stream gives every rank
  * the global result; its output may not feed another node.  When the graph
@@ -955,9 +956,8 @@ m3_status m3_cuda_abs_max_static(int device, void *stream, m3_dtype dtype,
  * the F32 range or comes near its lower end; a y below 2^-126 may be 0).
  * The row sums run in F32 in a fixed order of their own (not the reference's
  * left-to-right order of M3_OP_RMS_NORM; no chain of F32 additions is longer than
- * 300), so results repeat bit for bit; a row
- * whose squares pass the F32 range has y = 0 wherever h and scale are finite, as
- * its infinite mean says.
+ * 300), so results repeat bit for bit; a row whose squares pass the F32 range
+ * has y = 0 wherever h and scale are finite, as its infinite mean says.
  * `sum` (may be NULL) receives h.  It may be the very tensor `input` or
  * `residual` (same address and row stride); no other output may overlap an
  * input or another output (M3_STATUS_INVALID_ARGUMENT; the byte spans are

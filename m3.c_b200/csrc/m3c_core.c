@@ -101,8 +101,8 @@ bool m3c_dtype_float(m3_dtype dtype)
 }
 
 /* Same contract and statuses as the reference's m3_tensor_metadata_init
- * (src/m3_tensor.c:39-102): a known dtype (or the extension E4M3), rank <= 8, element and byte counts
- * without overflow. */
+ * (src/m3_tensor.c:39-102): a known dtype (or the extension E4M3), rank <= 8,
+ * element and byte counts without overflow. */
 m3_status m3c_metadata_init(m3_tensor_metadata *metadata, m3_dtype dtype,
                             uint8_t rank, const uint64_t *shape,
                             m3_error *error)

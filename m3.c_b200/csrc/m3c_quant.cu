@@ -350,7 +350,9 @@ __device__ __forceinline__ float norm_anew(const m3c_norm_e4m3_params &p, float 
 // of the groups that left the range, made anew from h.  Rare, so nothing is kept for
 // it from the pass before, and each thread reads its groups for itself (the warps
 // of a row that is one group share the reading).  The row's h, if it was stored, is
-// visible to it: a barrier of the row's warps is behind the stores.
+// visible to it: a barrier of the row's warps is behind the stores.  A function of its
+// own, so that the quick path's registers stay as they are (the variants of 32
+// registers spill 12 bytes for the call).
 template <bool ROW>
 __device__ __noinline__ void norm_anew_codes(const m3c_norm_e4m3_params &p, float inverse, uint32_t run)
 {

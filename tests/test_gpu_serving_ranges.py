@@ -179,6 +179,31 @@ def test_norm_products_past_the_range(m3, gpu, dtype, width, group, h, weight, e
         assert torch.equal(total, stored)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows, width, group", [
+    # one to eight pieces a thread of each kind, rows that share a CTA
+    (2050, 1040, 1040), (2050, 4104, 4104), (5, 16384, 16384), (5, 16384, 512), (5, 16384, 8192), (5, 16376, 16376),
+    (9, 516, 4), (5, 6001, 6001), (7, 256, 32), (7, 240, 24), (30, 40, 40), (30, 7, 7),
+])
+def test_norm_products_past_the_range_in_every_depth(m3, gpu, dtype, rows, width, group):
+    """As above, with rows and groups that stay in range between those that do not, and the sum in place."""
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(rows + width)
+    t = torch_dtype(dtype)
+    small, weight = (2.0 ** -14, 1e-38) if dtype == "f16" else (1e-25, 1e-22)
+    x = torch.randn(rows, width, generator=g, device="cuda")
+    x[1::3] *= small
+    x, r = x.to(t), (0.5 * x.roll(1, 1)).to(t)
+    w = torch.randn(width, generator=g, device="cuda")
+    w[width // 2:] *= weight
+    stored = (x.float() + r.float()).to(t)
+    total = x.clone()
+    codes, scales = run_norm(m3, total, w, group, r, total, epsilon=1e-36)
+    assert not check_norm_ranges(stored, w, group, codes, scales, 1e-36).any()
+    assert torch.equal(total, stored)
+
+
 def test_norm_zero_rows_with_a_small_epsilon(m3, gpu):
     import torch
 
